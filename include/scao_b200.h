@@ -407,6 +407,50 @@ SCAO_API int scao_wait_timeout_check(int* err, unsigned int limit, void* stream)
 SCAO_API int scao_divc_check(const float* x, const float* c, int n, int* mismatches,
                              void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* Operators of the training step around the optimizer                     */
+/* ---------------------------------------------------------------------- */
+
+/* Global norm of many gradients and clipping by it.  `table` (host): n rows
+ * of {device address, number of values, dtype}.  kind: the norm.  The norm of
+ * no values is 0; a NaN anywhere makes it NaN.  Accumulated in 64 bits,
+ * written as one float; the same inputs give the same bits.                */
+#define SCAO_NORM_1 0
+#define SCAO_NORM_2 1
+#define SCAO_NORM_INF 2
+SCAO_API int64_t scao_grad_norm_workspace_bytes(int n);
+SCAO_API int scao_grad_norm(const int64_t* table, int n, int kind, void* workspace,
+                            float* total, void* stream);
+/* g <- g min(1, max_norm / (*total + 1e-6)) for every gradient, rounded to
+ * its type once; nothing is written where the factor is 1.  The gradients
+ * must not share memory (scao_grads_overlap, host only: 1 if they do, -1 for
+ * a bad table).                                                            */
+SCAO_API int scao_grad_clip(const int64_t* table, int n, double max_norm, const float* total,
+                            void* stream);
+/* Both in one: the norm to *total, then the scaling by it.                 */
+SCAO_API int scao_grad_norm_clip(const int64_t* table, int n, int kind, double max_norm,
+                                 void* workspace, float* total, void* stream);
+SCAO_API int scao_grads_overlap(const int64_t* table, int n);
+
+/* Rotary positions of up to two tensors (queries and keys; heads[1] = 0 for
+ * one), each batch x heads x len x head_dim with strides in values for the
+ * first three and 1 for the last.  `turns` (host): dim / 2 frequencies in
+ * turns per position.  positions (device, int32 or int64, strides in values)
+ * or null: start + index.  inverse: the transposed rotation.               */
+typedef struct {
+    const void* in[2];
+    void* out[2];
+    int64_t in_stride[2][3], out_stride[2][3];
+    const double* turns;
+    const void* positions;
+    int64_t pos_stride_b, pos_stride_t, start;
+    int32_t heads[2];
+    int32_t dtype, batch, len, head_dim, dim, interleaved, positions_64, inverse;
+    float factor;
+    int32_t pad0;
+} ScaoRotary;
+SCAO_API int scao_rotary(const ScaoRotary* args, void* stream);
+
 /* Library identification. */
 SCAO_API const char* scao_version(void);
 

@@ -97,6 +97,19 @@ class PlanDev(C.Structure):
     ]
 
 
+class RotaryArgs(C.Structure):          # ScaoRotary
+    _fields_ = [
+        ("src", _P * 2), ("dst", _P * 2),
+        ("src_stride", (C.c_int64 * 3) * 2), ("dst_stride", (C.c_int64 * 3) * 2),
+        ("turns", _P), ("positions", _P),
+        ("pos_stride_b", C.c_int64), ("pos_stride_t", C.c_int64), ("start", C.c_int64),
+        ("heads", C.c_int32 * 2),
+        ("dtype", C.c_int32), ("batch", C.c_int32), ("len", C.c_int32), ("head_dim", C.c_int32),
+        ("dim", C.c_int32), ("interleaved", C.c_int32), ("positions_64", C.c_int32),
+        ("inverse", C.c_int32), ("factor", C.c_float), ("pad0", C.c_int32),
+    ]
+
+
 def check_layout():
     assert PARAM_DT.itemsize == 56, PARAM_DT.itemsize
     assert STEP_DT.itemsize == 128, STEP_DT.itemsize
@@ -105,6 +118,7 @@ def check_layout():
     assert STRIP_DT.itemsize == 24, STRIP_DT.itemsize
     assert FILTER_PARAM_DT.itemsize == 80, FILTER_PARAM_DT.itemsize
     assert C.sizeof(FilterDev) == 120, C.sizeof(FilterDev)
+    assert C.sizeof(RotaryArgs) == 216, C.sizeof(RotaryArgs)
 
 
 check_layout()
@@ -138,6 +152,12 @@ SIGNATURES = {
     "scao_plan_step": (C.c_int, [C.POINTER(PlanDev), _P]),
     "scao_plan_prep_factors": (C.c_int, [C.POINTER(PlanDev), _P, C.c_int, _P]),
     "scao_plan_lookahead": (C.c_int, [C.POINTER(PlanDev), C.c_float, C.c_int, _P]),
+    "scao_grad_norm_workspace_bytes": (C.c_int64, [C.c_int]),
+    "scao_grad_norm": (C.c_int, [_P, C.c_int, C.c_int, _P, _P, _P]),
+    "scao_grad_clip": (C.c_int, [_P, C.c_int, C.c_double, _P, _P]),
+    "scao_grad_norm_clip": (C.c_int, [_P, C.c_int, C.c_int, C.c_double, _P, _P, _P]),
+    "scao_grads_overlap": (C.c_int, [_P, C.c_int]),
+    "scao_rotary": (C.c_int, [C.POINTER(RotaryArgs), _P]),
     "scao_version": (C.c_char_p, []),
     "scao_divc_check": (C.c_int, [_P, _P, C.c_int, _P, _P]),
     "scao_tc_selftest": (C.c_int, [_P, _P, _P, C.c_int, C.c_int, _P, C.c_int, _P]),

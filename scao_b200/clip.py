@@ -1,0 +1,181 @@
+"""Global gradient norm and clipping, over any number of gradients in two launches.
+
+``clip_grad_norm_``, ``get_total_norm`` and ``clip_grads_with_norm_`` take what the
+functions of the same names in ``torch.nn.utils`` take (norms of order 1, 2 and inf)
+and return the norm as a float32 scalar on the gradients' device; nothing waits for
+the GPU.  Gradients may mix float32, bfloat16 and float16, sizes and alignments.
+Sums are held in 64 bits over the whole range of float32, the same inputs give the
+same bits, and each scaled value is rounded once.  Gradients within the threshold are
+not written.  CUDA tensors of one device only; errors raise.
+"""
+from __future__ import annotations
+
+import math
+from array import array
+
+import torch
+
+from . import _lib
+from .cuda import _CODE, _stream
+
+_KIND = {1.0: 0, 2.0: 1, math.inf: 2}
+
+
+def _layout(t):
+    """(dense, overlapping) of a strided tensor: its values fill a range of memory /
+    two of its elements may share an address."""
+    expected, dense = 1, True
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n != 1):
+        if stride < expected:
+            return False, True
+        dense = dense and stride == expected
+        expected += stride * (size - 1)
+    return dense, False
+
+
+def _table(tensors, write):
+    """(rows of the C table, tensors behind them, [(strided gradient, its packed copy)],
+    device).  Strided gradients that are not dense are packed for the call; tensors
+    that will be written must not share memory."""
+    dev = tensors[0].device
+    rows, kept, packed = [], [], []
+    for t in tensors:
+        if t.layout != torch.strided:
+            raise TypeError(f"unsupported gradient layout {t.layout}")
+        code = _CODE.get(t.dtype)
+        if code is None:
+            raise TypeError(f"unsupported gradient dtype {t.dtype}")
+        if t.device != dev:
+            raise ValueError(f"the gradients must be on one device, not {dev} and {t.device}")
+        if not t.is_contiguous():
+            dense, overlapping = _layout(t)
+            if overlapping and write:
+                raise ValueError("a gradient shares memory with itself (an expanded view): "
+                                 "it cannot be scaled in place")
+            if not dense:
+                packed.append((t, t.contiguous()))
+                t = packed[-1][1]
+        rows += (t.data_ptr(), t.numel(), code)
+        kept.append(t)
+    table = array("q", rows)
+    if write:
+        rc = _lib.lib().scao_grads_overlap(table.buffer_info()[0], len(tensors))
+        if rc == 1:
+            raise ValueError("two gradients share memory: each can be scaled only once")
+        _lib.check(rc, "scao_grads_overlap")
+    if dev.type != "cuda":
+        raise RuntimeError("scao_b200: gradients must be CUDA tensors (no CPU path)")
+    return table, kept, packed, dev
+
+
+def _kind(norm_type):
+    kind = _KIND.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, not {norm_type}")
+    return kind
+
+
+def _max_norm(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be at least 0, not {max_norm}")
+    return max_norm
+
+
+def _grads(parameters):
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return [p.grad for p in parameters if p.grad is not None]
+
+
+def _refuse_nonfinite(total, norm_type):
+    if not bool(torch.isfinite(total)):
+        raise RuntimeError(f"the total norm of order {norm_type} of the gradients is not finite, "
+                           "so they cannot be clipped; pass error_if_nonfinite=False to scale "
+                           "by it all the same")
+
+
+def _workspace(n, dev):
+    size = int(_lib.lib().scao_grad_norm_workspace_bytes(n))
+    return torch.empty(size, dtype=torch.uint8, device=dev)
+
+
+def _finish(grads, packed):
+    for g, copy in packed:
+        g.copy_(copy)
+    torch.autograd.graph.increment_version([g for g in grads if not g.is_inference()])
+
+
+@torch.no_grad()
+def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False):
+    """The norm of all values of ``tensors`` (a tensor or an iterable) as if they were
+    one vector: a float32 scalar on their device.  ``norm_type`` is 1, 2 or inf;
+    no tensors give 0, a NaN anywhere gives NaN.  ``error_if_nonfinite`` waits for the
+    GPU and raises where the norm is inf or NaN."""
+    kind = _kind(norm_type)
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    table, _kept, _, dev = _table(tensors, write=False)
+    n = len(tensors)
+    total = torch.empty((), dtype=torch.float32, device=dev)
+    ws = _workspace(n, dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().scao_grad_norm(table.buffer_info()[0], n, kind, ws.data_ptr(),
+                                             total.data_ptr(), _stream(dev)), "scao_grad_norm")
+    if error_if_nonfinite:
+        _refuse_nonfinite(total, norm_type)
+    return total
+
+
+@torch.no_grad()
+def clip_grads_with_norm_(parameters, max_norm, total_norm):
+    """Scales the gradients of ``parameters`` (a tensor or an iterable) in place by
+    min(1, max_norm / (total_norm + 1e-6)); ``total_norm`` is a scalar tensor on their
+    device, as ``get_total_norm`` returns it (or reduced over ranks)."""
+    max_norm = _max_norm(max_norm)
+    grads = _grads(parameters)
+    if not grads or max_norm == math.inf:
+        return
+    table, _kept, packed, dev = _table(grads, write=True)
+    if total_norm.numel() != 1 or total_norm.device != dev:
+        raise ValueError("total_norm must be one number on the gradients' device")
+    total = total_norm.to(torch.float32)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().scao_grad_clip(table.buffer_info()[0], len(grads), max_norm,
+                                             total.data_ptr(), _stream(dev)), "scao_grad_clip")
+    _finish(grads, packed)
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Clips the gradients of ``parameters`` (a tensor or an iterable) in place so that
+    their norm, taken over all of them as one vector, is at most ``max_norm``:
+    g <- g min(1, max_norm / (norm + 1e-6)).  Returns the norm before clipping, a
+    float32 scalar on their device.  ``norm_type`` is 1, 2 or inf; an infinite
+    ``max_norm`` leaves the gradients as they are; a norm that is NaN makes every
+    gradient NaN unless ``error_if_nonfinite``, which waits for the GPU and raises
+    before anything is scaled.  Two gradients that share memory are refused."""
+    kind, max_norm = _kind(norm_type), _max_norm(max_norm)
+    grads = _grads(parameters)
+    if not grads:
+        return torch.tensor(0.0)
+    if max_norm == math.inf:
+        return get_total_norm(grads, norm_type, error_if_nonfinite)
+    table, _kept, packed, dev = _table(grads, write=True)
+    n = len(grads)
+    total = torch.empty((), dtype=torch.float32, device=dev)
+    ws = _workspace(n, dev)
+    L, at = _lib.lib(), table.buffer_info()[0]
+    with torch.cuda.device(dev):
+        if error_if_nonfinite:
+            _lib.check(L.scao_grad_norm(at, n, kind, ws.data_ptr(), total.data_ptr(), _stream(dev)),
+                       "scao_grad_norm")
+            _refuse_nonfinite(total, norm_type)
+            _lib.check(L.scao_grad_clip(at, n, max_norm, total.data_ptr(), _stream(dev)),
+                       "scao_grad_clip")
+        else:
+            _lib.check(L.scao_grad_norm_clip(at, n, kind, max_norm, ws.data_ptr(), total.data_ptr(),
+                                             _stream(dev)), "scao_grad_norm_clip")
+    _finish(grads, packed)
+    return total

@@ -13,6 +13,7 @@ enum ScaoSlot {
     SLOT_GRAM_EMA, SLOT_REQUANT, SLOT_DIAG_EMA, SLOT_EIG_PREP, SLOT_EIG_DIAG,
     SLOT_EIG_GEMM, SLOT_EIG_JACOBI, SLOT_EIG_RESIDUAL, SLOT_EIG_CHOLINV, SLOT_EIG_RANK,
     SLOT_QUANT, SLOT_SEAM, SLOT_GRAM_TC, SLOT_TRANSPOSE, SLOT_FILTER, SLOT_EIG_ITER,
+    SLOT_CLIP, SLOT_ROTARY, SLOT_GATED_FF,
     SLOT_COUNT
 };
 

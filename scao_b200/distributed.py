@@ -26,6 +26,8 @@ import heapq
 import torch
 import torch.distributed as dist
 
+from .clip import _max_norm, clip_grads_with_norm_, get_total_norm
+
 ALIGN = 64   # elements: every parameter slot starts on a 128-byte boundary
 
 
@@ -348,8 +350,29 @@ class ShardedSCAO:
                 o._norm_average = (lambda a, c: (lambda _live: (a, c)))(avg, n)
         return avg
 
+    # clipping by the global norm -------------------------------------------
+    def _clip(self, max_norm):
+        """Scales this rank's averaged gradients by the norm over all
+        parameters: the owners' sums of squares meet in one all-reduce of a
+        64-bit number.  Returns the norm before clipping, the same on every
+        rank."""
+        mine = [self.params[i] for i in self.my]
+        square = torch.zeros(1, dtype=torch.float64, device=self.device)
+        if mine:
+            square += get_total_norm([p.grad for p in mine]).double().square()
+        dist.all_reduce(square, group=self.group)
+        total = square.sqrt().float().reshape(())
+        clip_grads_with_norm_(mine, max_norm, total)
+        return total
+
     # step -------------------------------------------------------------------
-    def step(self):
+    def step(self, max_grad_norm=None):
+        """``max_grad_norm``: clip the averaged gradients by their global norm
+        (order 2, over all ranks' parameters) first; ``total_norm`` then holds
+        the norm before clipping.  The norm needs every bucket, so no bucket
+        steps before the last gradient is reduced."""
+        if max_grad_norm is not None:
+            max_grad_norm = _max_norm(max_grad_norm)
         self.global_step += 1
         hooked = getattr(self, "_pending", None) is not None
         if hooked:
@@ -357,12 +380,12 @@ class ShardedSCAO:
         if self.cur is None:
             raise RuntimeError("no gradients staged (load_grads / flat_grad_from_params)")
         try:
-            self._step(hooked)
+            self._step(hooked, max_grad_norm)
         finally:
             if hooked:
                 self._pending = None
 
-    def _step(self, hooked):
+    def _step(self, hooked, max_grad_norm=None):
         nb = self.layout.nb
         if not self.nccl:
             for b in range(nb):
@@ -373,6 +396,8 @@ class ShardedSCAO:
                 dist.all_reduce(tmp, group=self.group)
                 seg = self.layout.seg[b]
                 mine_g.copy_(tmp[self.rank * seg:(self.rank + 1) * seg] / self.world)
+            if max_grad_norm is not None:
+                self.total_norm = self._clip(max_grad_norm)
             if self.norm_sync:
                 self._share_norm_average()
             for b in range(nb):
@@ -397,10 +422,13 @@ class ShardedSCAO:
                         dist.reduce_scatter_tensor(mine_g, full_g, op=dist.ReduceOp.AVG,
                                                    group=self.group)
                     ev_rs[b].record(C)
-        if self.norm_sync:
-            # the average needs every bucket's gradients: no step starts before
+        if self.norm_sync or max_grad_norm is not None:
+            # both norms need every bucket's gradients: no step starts before
             for b in range(nb):
                 D.wait_event(ev_rs[b])
+        if max_grad_norm is not None:
+            self.total_norm = self._clip(max_grad_norm)
+        if self.norm_sync:
             self._share_norm_average()
         for b in range(nb):
             D.wait_event(ev_rs[b])

@@ -23,6 +23,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .clip import clip_grad_norm_
+
 
 @dataclass
 class GPTConfig:
@@ -104,14 +106,21 @@ def loss_fn(model, tokens):
                            tokens[:, 1:].reshape(-1))
 
 
-def train_step(model, opt, tokens, sharded=None):
-    """Forward + backward (bf16 autocast) + SCAO step; returns the loss."""
+def train_step(model, opt, tokens, sharded=None, max_grad_norm=None):
+    """Forward + backward (bf16 autocast) + SCAO step; returns the loss.
+    ``max_grad_norm`` clips the gradients by their global norm before the step
+    (across ranks: the averaged gradients, by the norm over all of them)."""
     loss = loss_fn(model, tokens)
     loss.backward()
     if sharded is not None:
         sharded.flat_grad_from_params()
-        sharded.step()
+        if max_grad_norm is None:
+            sharded.step()
+        else:
+            sharded.step(max_grad_norm)
     else:
+        if max_grad_norm is not None:
+            clip_grad_norm_(model.parameters(), max_grad_norm)
         opt.step()
     model.zero_grad(set_to_none=True)
     return loss.detach()

@@ -1,0 +1,177 @@
+"""Rotary positions for attention queries and keys, forward and backward, one launch each.
+
+    rotary = Rotary(64)                       # values turned per head, base 10000
+    q, k = rotary(q, k)                       # (batch, heads, length, head_dim)
+    q, k = rotary(q, k, positions=cached)     # continue at position `cached`
+    q, k = rotary(q, k, positions=ids)        # integer tensor (length) or (batch, length)
+
+Pair j of a head at position p turns by p w_j, w_j = base^(-2j / dim); the pair is
+(2j, 2j + 1) where ``interleaved``, else (j, j + dim / 2); values from ``dim`` on pass
+through.  Angles are formed in 64 bits, so far positions stay exact.  Any strides with
+neighbouring values of a head next to each other are read as they are (views of a fused
+projection, (batch, length, heads, head_dim) memory).  float32, bfloat16 and float16,
+CUDA tensors of one device.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .cuda import _CODE, _on_cuda, _stream
+
+MAX_DIM = 512
+
+
+@dataclass(frozen=True)
+class RotaryScaling:
+    """Frequencies for contexts ``factor`` times as long as the trained one.
+
+    * ``"linear"``: every frequency divided by ``factor`` (position interpolation);
+    * ``"ntk"``: base multiplied by factor^(dim / (dim - 2)), so the slowest pair is
+      divided by ``factor`` and the fastest is kept;
+    * ``"yarn"``: per frequency, by the turns r it makes over ``original_len``: kept where
+      r >= ``fast``, divided by ``factor`` where r <= ``slow``, and the mean of both
+      weighted by (r - slow) / (fast - slow) between; the turned values are multiplied by
+      ``magnitude`` (0.1 ln(factor) + 1 where that is None).
+    """
+    kind: str
+    factor: float
+    original_len: int | None = None
+    fast: float = 32.0
+    slow: float = 1.0
+    magnitude: float | None = None
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "ntk", "yarn"):
+            raise ValueError(f"rotary scaling must be linear, ntk or yarn, not {self.kind!r}")
+        if not (math.isfinite(self.factor) and self.factor >= 1):
+            raise ValueError(f"rotary scaling factor must be at least 1, not {self.factor}")
+        if self.kind == "yarn":
+            if self.original_len is None or self.original_len < 1:
+                raise ValueError("yarn scaling needs original_len, the trained context length")
+            if not 0 <= self.slow < self.fast:
+                raise ValueError("yarn scaling needs 0 <= slow < fast")
+
+
+def _frequencies(dim, base, s):
+    """(radians per position of each pair, factor on the turned values)."""
+    if s is not None and s.kind == "ntk":
+        if dim == 2:
+            raise ValueError("ntk scaling needs dim > 2")
+        base = base * s.factor ** (dim / (dim - 2))
+    freq = [base ** (-2.0 * j / dim) for j in range(dim // 2)]
+    if s is None or s.kind == "ntk":
+        return freq, 1.0
+    if s.kind == "linear":
+        return [w / s.factor for w in freq], 1.0
+    keep = [min(max((s.original_len * w / (2 * math.pi) - s.slow) / (s.fast - s.slow), 0.0), 1.0)
+            for w in freq]
+    magnitude = 0.1 * math.log(s.factor) + 1.0 if s.magnitude is None else s.magnitude
+    return [w * m + w / s.factor * (1 - m) for w, m in zip(freq, keep)], magnitude
+
+
+class Rotary:
+    """Rotary positions over the first ``dim`` values of each head (module docstring)."""
+
+    def __init__(self, dim, base=10000.0, *, interleaved=False, scaling=None):
+        if dim < 2 or dim % 2 or dim > MAX_DIM:
+            raise ValueError(f"rotary dim must be even and within 2..{MAX_DIM}, not {dim}")
+        if not (math.isfinite(base) and base > 0):
+            raise ValueError(f"rotary base must be positive, not {base}")
+        self.dim, self.base, self.interleaved, self.scaling = dim, float(base), bool(interleaved), scaling
+        self.frequencies, self.magnitude = _frequencies(dim, self.base, scaling)
+        self._turns = (ctypes.c_double * (dim // 2))(*[w / (2 * math.pi) for w in self.frequencies])
+
+    def __call__(self, q, k=None, positions=None):
+        """The turned q, or (q, k): new tensors of the same shape, type and order in
+        memory.  ``positions``: None counts from 0, an int from there, an integer tensor
+        gives each token's, (length) or (batch, length)."""
+        for name, t in (("q", q), ("k", k)):
+            if t is None:
+                continue
+            if t.dim() != 4:
+                raise ValueError(f"{name} must be (batch, heads, length, head_dim), not {tuple(t.shape)}")
+            if t.dtype not in _CODE:
+                raise TypeError(f"unsupported dtype {t.dtype}")
+            if t.shape[3] < self.dim:
+                raise ValueError(f"head_dim {t.shape[3]} is below the rotary dim {self.dim}")
+        if k is not None and (k.dtype != q.dtype or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]):
+            raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must share "
+                             "batch, length, head_dim and dtype")
+        start = 0
+        if isinstance(positions, torch.Tensor):
+            if positions.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"positions must be int32 or int64, not {positions.dtype}")
+            if positions.dim() not in (1, 2) or positions.shape[-1] != q.shape[2] or \
+                    (positions.dim() == 2 and positions.shape[0] not in (1, q.shape[0])):
+                raise ValueError(f"positions {tuple(positions.shape)} do not fit q {tuple(q.shape)}")
+        elif positions is not None:
+            start, positions = int(positions), None
+            if abs(start) >= 1 << 52:
+                raise ValueError(f"position {start} is out of range")
+        dev = _on_cuda(q, *(t for t in (k, positions) if isinstance(t, torch.Tensor)))
+        out = _Turn.apply(self, False, positions, start, dev, q, k)
+        return out[0] if k is None else out
+
+
+def _strides(t):
+    """Batch, head and token strides; 0 where there is one only."""
+    return [st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride()[:3])]
+
+
+def _run(rotary, inverse, positions, start, dev, tensors):
+    """The turned tensors (None stays None)."""
+    a = _lib.RotaryArgs()
+    outs, kept = [], []
+    for i, x in enumerate(tensors):
+        if x is None:
+            outs.append(None)
+            continue
+        if x.stride(3) != 1:
+            x = x.contiguous()
+        y = torch.empty_like(x)
+        if y.stride(3) != 1:
+            y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        a.src[i], a.dst[i] = x.data_ptr(), y.data_ptr()
+        a.src_stride[i][:], a.dst_stride[i][:] = _strides(x), _strides(y)
+        a.heads[i] = x.shape[1]
+        a.dtype, a.batch, a.len, a.head_dim = _CODE[x.dtype], x.shape[0], x.shape[2], x.shape[3]
+        outs.append(y)
+        kept.append(x)
+    a.turns = ctypes.addressof(rotary._turns)
+    a.dim, a.interleaved, a.inverse = rotary.dim, rotary.interleaved, inverse
+    a.factor, a.start = rotary.magnitude, start
+    if positions is not None:
+        a.positions, a.positions_64 = positions.data_ptr(), positions.dtype == torch.int64
+        a.pos_stride_t = positions.stride(-1) if positions.shape[-1] > 1 else 0
+        a.pos_stride_b = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    if kept:
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().scao_rotary(ctypes.byref(a), _stream(dev)), "scao_rotary")
+    return outs
+
+
+class _Turn(torch.autograd.Function):
+    """The rotation, or its transpose (``inverse``), which is its gradient."""
+
+    @staticmethod
+    def forward(ctx, rotary, inverse, positions, start, dev, q, k):
+        ctx.args = rotary, inverse, start, dev
+        ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
+        return tuple(_run(rotary, inverse, positions, start, dev, (q, k)))
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        rotary, inverse, start, dev = ctx.args
+        (positions,) = ctx.saved_tensors
+        if not ctx.needs_input_grad[5]:
+            gq = None
+        if not ctx.needs_input_grad[6]:
+            gk = None
+        gq, gk = _Turn.apply(rotary, not inverse, positions, start, dev, gq, gk)
+        return None, None, None, None, None, gq, gk

@@ -1,0 +1,158 @@
+"""Refusals and host logic of the operators around the optimizer step; no GPU."""
+import ctypes
+import math
+from array import array
+
+import pytest
+import torch
+
+from scao_b200 import (Rotary, RotaryScaling, _lib, clip_grad_norm_, clip_grads_with_norm_,
+                       get_total_norm)
+from scao_b200.clip import _layout
+
+
+def param(grad):
+    p = torch.nn.Parameter(torch.empty(grad.shape, dtype=grad.dtype))
+    p.grad = grad
+    return p
+
+
+# ------------------------------------------------------------------- clipping
+@pytest.mark.parametrize("norm_type", [0, 3, 0.5, -1, math.nan, -math.inf])
+def test_clip_refuses_norms(norm_type):
+    with pytest.raises(ValueError, match="norm_type"):
+        clip_grad_norm_([param(torch.ones(3))], 1.0, norm_type)
+    with pytest.raises(ValueError, match="norm_type"):
+        get_total_norm([torch.ones(3)], norm_type)
+
+
+@pytest.mark.parametrize("max_norm", [-1.0, math.nan, -math.inf])
+def test_clip_refuses_thresholds(max_norm):
+    with pytest.raises(ValueError, match="max_norm"):
+        clip_grad_norm_([param(torch.ones(3))], max_norm)
+    with pytest.raises(ValueError, match="max_norm"):
+        clip_grads_with_norm_([param(torch.ones(3))], max_norm, torch.ones(()))
+
+
+def test_clip_refuses_types_and_devices():
+    with pytest.raises(TypeError, match="dtype"):
+        clip_grad_norm_([param(torch.ones(3, dtype=torch.float64))], 1.0)
+    with pytest.raises(TypeError, match="layout"):
+        get_total_norm([torch.eye(3).to_sparse()])
+    with pytest.raises(ValueError, match="one device"):
+        get_total_norm([torch.ones(3), torch.ones(3, device="meta")])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        clip_grad_norm_([param(torch.ones(3))], 1.0)
+
+
+def test_clip_refuses_shared_memory():
+    base = torch.ones(20)
+    for a, b in ((base[:10], base[9:]), (base, base), (base[3:5], base)):
+        with pytest.raises(ValueError, match="share memory"):
+            clip_grad_norm_([param(a), param(b)], 1.0)
+    with pytest.raises(ValueError, match="with itself"):
+        clip_grad_norm_([param(torch.ones(1).expand(5))], 1.0)
+    with pytest.raises(RuntimeError, match="CUDA"):            # neighbours do not share
+        clip_grad_norm_([param(base[:10]), param(base[10:])], 1.0)
+
+
+def test_clip_without_gradients():
+    assert clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0).item() == 0
+    assert clip_grads_with_norm_([], 1.0, torch.ones(())) is None
+
+
+@pytest.mark.parametrize("view,want", [
+    (lambda x: x, (True, False)), (lambda x: x.t(), (True, False)), (lambda x: x[:, 1:], (False, False)),
+    (lambda x: x[::2], (False, False)), (lambda x: x[:1].expand(4, 6), (False, True)),
+    (lambda x: x.as_strided((4, 4), (2, 1)), (False, True)), (lambda x: x[:, :1], (False, False)),
+    (lambda x: x[1:2], (True, False))])
+def test_layout(view, want):
+    assert _layout(view(torch.zeros(8, 6))) == want
+
+
+def test_clip_c_entry_checks():
+    L = _lib.lib()
+    bad = [(0, 5, 0), (4096, -1, 0), (4096, 5, 3), (4097, 5, 0), (4096, 1 << 48, 0)]
+    for row in bad:
+        t = array("q", row)
+        assert L.scao_grads_overlap(t.buffer_info()[0], 1) == -1
+        assert L.scao_grad_norm(t.buffer_info()[0], 1, 1, 4096, 4096, None) == 1
+    t = array("q", (4096, 5, 0, 4096 + 20, 3, 1, 0, 0, 0))
+    assert L.scao_grads_overlap(t.buffer_info()[0], 3) == 0
+    t[3] = 4096 + 18
+    assert L.scao_grads_overlap(t.buffer_info()[0], 3) == 1
+    assert L.scao_grad_norm(t.buffer_info()[0], 3, 7, 4096, 4096, None) == 1       # no such norm
+    assert L.scao_grad_norm(t.buffer_info()[0], 3, 1, 4096, None, None) == 1       # nowhere to write
+    assert L.scao_grad_norm_clip(t.buffer_info()[0], 3, 1, -1.0, 4096, 4096, None) == 1
+    assert L.scao_grad_norm_workspace_bytes(1) <= L.scao_grad_norm_workspace_bytes(5000)
+
+
+# -------------------------------------------------------------------- rotary
+@pytest.mark.parametrize("dim", [0, 1, 3, -2, 514])
+def test_rotary_refuses_dims(dim):
+    with pytest.raises(ValueError, match="dim"):
+        Rotary(dim)
+
+
+@pytest.mark.parametrize("make", [
+    lambda: Rotary(8, base=0.0), lambda: Rotary(8, base=math.inf), lambda: RotaryScaling("cubic", 2.0),
+    lambda: RotaryScaling("linear", 0.5), lambda: RotaryScaling("linear", math.nan),
+    lambda: RotaryScaling("yarn", 2.0), lambda: RotaryScaling("yarn", 2.0, original_len=0),
+    lambda: RotaryScaling("yarn", 2.0, original_len=9, fast=1, slow=2),
+    lambda: Rotary(2, scaling=RotaryScaling("ntk", 2.0))])
+def test_rotary_refuses_settings(make):
+    with pytest.raises(ValueError):
+        make()
+
+
+def test_rotary_refuses_tensors():
+    r = Rotary(8)
+    q = torch.zeros(2, 3, 5, 8)
+    for args in ((q[0],), (q[..., :6],), (q, q[:1]), (q, q[:, :, :4]), (q, q.double().float()[..., :7]),
+                 (q, q.half())):
+        with pytest.raises(ValueError):
+            r(*args)
+    with pytest.raises(TypeError, match="dtype"):
+        r(q.double())
+    for p in (torch.zeros(4, dtype=torch.long), torch.zeros(3, 5, dtype=torch.long),
+              torch.zeros(1, 1, 5, dtype=torch.long), 1 << 60):
+        with pytest.raises(ValueError):
+            r(q, positions=p)
+    with pytest.raises(TypeError, match="int32 or int64"):
+        r(q, positions=torch.zeros(5))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        r(q)
+
+
+def test_rotary_frequencies():
+    plain = Rotary(64).frequencies
+    assert plain[0] == 1.0 and math.isclose(plain[-1], 10000 ** (-62 / 64))
+    ntk = Rotary(64, scaling=RotaryScaling("ntk", 8.0)).frequencies
+    assert ntk[0] == 1.0 and math.isclose(ntk[-1], plain[-1] / 8)
+    yarn = Rotary(64, scaling=RotaryScaling("yarn", 8.0, original_len=8192))
+    assert yarn.frequencies[0] == plain[0] and math.isclose(yarn.frequencies[-1], plain[-1] / 8)
+    assert math.isclose(yarn.magnitude, 0.1 * math.log(8) + 1)
+    assert all(p / 8 <= y <= p for p, y in zip(plain, yarn.frequencies))
+
+
+def test_rotary_c_entry_checks():
+    L = _lib.lib()
+    turns = (ctypes.c_double * 4)(*[0.1] * 4)
+
+    def call(**kw):
+        a = _lib.RotaryArgs()
+        a.turns, a.dim, a.head_dim, a.batch, a.len, a.dtype = ctypes.addressof(turns), 8, 8, 1, 1, 0
+        a.heads[0] = 1
+        a.src[0] = a.dst[0] = 4096
+        for k, v in kw.items():
+            if k in ("src", "dst"):
+                getattr(a, k)[0] = v
+            else:
+                setattr(a, k, v)
+        return L.scao_rotary(ctypes.byref(a), None)
+
+    for kw in (dict(dim=7), dict(dim=0), dict(dim=10), dict(dtype=3), dict(batch=-1), dict(turns=None),
+               dict(src=None), dict(dst=4098)):
+        assert call(**kw) == 1, kw
+    assert call(batch=0) == 0
+    assert L.scao_rotary(None, None) == 1
