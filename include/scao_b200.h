@@ -39,6 +39,8 @@ extern "C" {
 #define SCAO_ERR_NOCONV 3     /* eigensolver hit its iteration cap (status
                                  per problem is also written to the device)  */
 
+#define SCAO_ERR_TIMEOUT 4    /* a bounded wait in an earlier kernel ran out  */
+
 /* parameter dtypes */
 #define SCAO_F32 0
 #define SCAO_BF16 1
@@ -450,6 +452,33 @@ typedef struct {
     int32_t pad0;
 } ScaoRotary;
 SCAO_API int scao_rotary(const ScaoRotary* args, void* stream);
+
+/* Gated feed-forward product h = act(x Wg^T) * (x Wu^T) of 16-bit matrices
+ * (SCAO_BF16 / SCAO_F16), x: rows x d, Wg and Wu: ff x d, h: rows x ff, with
+ * 32-bit sums.  x, w_gate, w_up start on 16 bytes and have row pitches ldx,
+ * ldg, ldu that are multiples of 8 values; h, dx, dw_gate, dw_up are packed.
+ * `saved` (scao_gated_ff_saved_bytes; null if no gradient will be taken)
+ * keeps what backward reads.  backward: from dh (row pitch lddh) to dx and to
+ * dw_gate and dw_up (null: not wanted, the two together), with a workspace
+ * of scao_gated_ff_workspace_bytes, 16-byte aligned.  A kernel whose wait
+ * ran out sets the status word (host memory; null where there is no GPU);
+ * the next call clears it and returns SCAO_ERR_TIMEOUT without launching.  */
+#define SCAO_ACT_SILU 0
+#define SCAO_ACT_GELU 1
+#define SCAO_ACT_GELU_TANH 2
+typedef struct {
+    const void *x, *w_gate, *w_up;
+    void *h, *saved;
+    const void* dh;
+    void *dx, *dw_gate, *dw_up, *workspace;
+    int64_t ldx, ldg, ldu, lddh;
+    int32_t rows, d, ff, dtype, act, pad0;
+} ScaoGatedFf;
+SCAO_API int64_t scao_gated_ff_saved_bytes(int rows, int ff);
+SCAO_API int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff);
+SCAO_API int* scao_gated_ff_status_word(void);
+SCAO_API int scao_gated_ff_forward(const ScaoGatedFf* args, void* stream);
+SCAO_API int scao_gated_ff_backward(const ScaoGatedFf* args, void* stream);
 
 /* Library identification. */
 SCAO_API const char* scao_version(void);

@@ -9,6 +9,7 @@ from . import logging as scao_logging
 from .sparse_preconditioner import SparsePreconditioner
 from .presets import scao_sub1b, scao_1b, scao_3b, scao_7b, scao_40b, scao_125b
 from .clip import clip_grad_norm_, clip_grads_with_norm_, get_total_norm
+from .feedforward import GatedFeedForward, gated_ff
 from .rotary import Rotary, RotaryScaling
 from .utils import (adaptive_rank, low_rank_matrix_power_neg_quarter, matrix_power_neg_quarter,
                     newton_schulz_root_inv)
@@ -18,4 +19,4 @@ __version__ = "0.1.0"
 __all__ = ["SCAO", "SparsePreconditioner", "scao_logging", "adaptive_rank", "matrix_power_neg_quarter", "newton_schulz_root_inv",
            "low_rank_matrix_power_neg_quarter", "scao_sub1b", "scao_1b", "scao_3b", "scao_7b",
            "scao_40b", "scao_125b", "clip_grad_norm_", "clip_grads_with_norm_", "get_total_norm",
-           "Rotary", "RotaryScaling", "__version__"]
+           "gated_ff", "GatedFeedForward", "Rotary", "RotaryScaling", "__version__"]

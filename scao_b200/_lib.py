@@ -110,6 +110,13 @@ class RotaryArgs(C.Structure):          # ScaoRotary
     ]
 
 
+class GatedFfArgs(C.Structure):         # ScaoGatedFf
+    _fields_ = [(n, _P) for n in ("x", "w_gate", "w_up", "h", "saved", "dh", "dx", "dw_gate", "dw_up",
+                                  "workspace")] + \
+               [(n, C.c_int64) for n in ("ldx", "ldg", "ldu", "lddh")] + \
+               [(n, C.c_int32) for n in ("rows", "d", "ff", "dtype", "act", "pad0")]
+
+
 def check_layout():
     assert PARAM_DT.itemsize == 56, PARAM_DT.itemsize
     assert STEP_DT.itemsize == 128, STEP_DT.itemsize
@@ -119,6 +126,7 @@ def check_layout():
     assert FILTER_PARAM_DT.itemsize == 80, FILTER_PARAM_DT.itemsize
     assert C.sizeof(FilterDev) == 120, C.sizeof(FilterDev)
     assert C.sizeof(RotaryArgs) == 216, C.sizeof(RotaryArgs)
+    assert C.sizeof(GatedFfArgs) == 136, C.sizeof(GatedFfArgs)
 
 
 check_layout()
@@ -158,6 +166,11 @@ SIGNATURES = {
     "scao_grad_norm_clip": (C.c_int, [_P, C.c_int, C.c_int, C.c_double, _P, _P, _P]),
     "scao_grads_overlap": (C.c_int, [_P, C.c_int]),
     "scao_rotary": (C.c_int, [C.POINTER(RotaryArgs), _P]),
+    "scao_gated_ff_saved_bytes": (C.c_int64, [C.c_int, C.c_int]),
+    "scao_gated_ff_workspace_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
+    "scao_gated_ff_status_word": (C.POINTER(C.c_int), []),
+    "scao_gated_ff_forward": (C.c_int, [C.POINTER(GatedFfArgs), _P]),
+    "scao_gated_ff_backward": (C.c_int, [C.POINTER(GatedFfArgs), _P]),
     "scao_version": (C.c_char_p, []),
     "scao_divc_check": (C.c_int, [_P, _P, C.c_int, _P, _P]),
     "scao_tc_selftest": (C.c_int, [_P, _P, _P, C.c_int, C.c_int, _P, C.c_int, _P]),
@@ -198,7 +211,13 @@ def lib():
     return L
 
 
+TIMEOUT = 4
+
+
 def check(rc, what):
+    if rc == TIMEOUT:
+        raise ScaoError(f"{what}: a completion wait in an earlier kernel timed out; "
+                        "its results are not valid")
     if rc != 0:
         raise ScaoError(f"{what} failed with status {rc}")
 

@@ -77,6 +77,21 @@ bool scao_build_tensor_maps(const ScaoPlanDev* P, const ScaoParam* ph, const Sca
                            cudaMemcpyHostToDevice, st) == cudaSuccess;
 }
 
+bool scao_tensor_map_2d(void* map, int dtype, const void* base, int64_t rows, int64_t cols, int64_t ld,
+                        int bx, int by) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)bx, (cuuint32_t)by};
+    const cuuint32_t estr[2] = {1, 1};
+    return enc((CUtensorMap*)map,
+               dtype == SCAO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+               (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int scao_sm_count() {
     static int n = 0;
     if (!n) {

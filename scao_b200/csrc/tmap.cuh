@@ -38,6 +38,12 @@ __host__ __device__ inline const void* scao_tmap(const uint8_t* base, int param,
     return base + ((size_t)param * TMA_PER_PARAM + slot) * 128;
 }
 
+// One map of a rows x cols matrix of 16-bit values (dtype SCAO_BF16 / SCAO_F16)
+// with row pitch ld (values; a multiple of 8, as the base is of 16 bytes): boxes of
+// by rows x bx columns, 128-byte swizzle, zero fill out of bounds.
+bool scao_tensor_map_2d(void* map, int dtype, const void* base, int64_t rows, int64_t cols, int64_t ld,
+                        int bx, int by);
+
 int scao_sm_count();
 
 // persistent-kernel grid: SMs minus the plan's reservation, at most `work`

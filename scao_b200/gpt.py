@@ -6,7 +6,10 @@ SCAO optimizer -- the caller of the optimizer step in benchmark configuration C3
 The architecture follows the reference's benchmark model
 (scao/benchmarks/gpt_scale_benchmark.py:79-170): fused bias-free QKV and
 output projections, bias-free GELU MLP, pre-LayerNorm blocks, learned
-positions, LM head tied to the token embedding, N(0, 0.02^2) init.
+positions, LM head tied to the token embedding, N(0, 0.02^2) init.  Beyond it,
+``GPTConfig`` takes a gated feed-forward block (``mlp="gated"``, with
+``activation``), rotary positions (``positions="rotary"``, with their base and
+scaling) and fewer key / value heads than query heads (``n_kv_head``).
 
 ``train_step`` runs forward / backward under bf16 autocast, then the SCAO step:
 on one GPU ``opt.step()``; across ranks the owner-compute ``ShardedSCAO``
@@ -24,6 +27,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .clip import clip_grad_norm_
+from .feedforward import GatedFeedForward
+from .rotary import Rotary, RotaryScaling
 
 
 @dataclass
@@ -34,6 +39,20 @@ class GPTConfig:
     d_ff: int = 4096
     vocab: int = 50257
     seq_len: int = 1024
+    mlp: str = "gelu"                   # or "gated": GatedFeedForward
+    activation: str = "silu"            # of the gated block
+    positions: str = "learned"          # or "rotary"
+    rotary_base: float = 10000.0
+    rotary_scaling: RotaryScaling | None = None
+    n_kv_head: int | None = None        # key / value heads; None: n_head
+
+    def __post_init__(self):
+        if self.mlp not in ("gelu", "gated"):
+            raise ValueError(f"mlp must be gelu or gated, not {self.mlp!r}")
+        if self.positions not in ("learned", "rotary"):
+            raise ValueError(f"positions must be learned or rotary, not {self.positions!r}")
+        if self.n_kv_head is not None and (self.n_kv_head < 1 or self.n_head % self.n_kv_head):
+            raise ValueError(f"n_head {self.n_head} is not a multiple of n_kv_head {self.n_kv_head}")
 
 
 GPT2_MEDIUM = GPTConfig()
@@ -43,14 +62,23 @@ class _Attention(nn.Module):
     def __init__(self, c: GPTConfig):
         super().__init__()
         self.n_head = c.n_head
-        self.qkv = nn.Linear(c.d_model, 3 * c.d_model, bias=False)
+        self.n_kv_head = c.n_kv_head or c.n_head
+        self.d_kv = c.d_model // c.n_head * self.n_kv_head
+        self.rotary = None
+        if c.positions == "rotary":
+            self.rotary = Rotary(c.d_model // c.n_head, c.rotary_base, scaling=c.rotary_scaling)
+        self.qkv = nn.Linear(c.d_model, c.d_model + 2 * self.d_kv, bias=False)
         self.proj = nn.Linear(c.d_model, c.d_model, bias=False)
 
     def forward(self, x):
         B, T, C = x.shape
-        q, k, v = self.qkv(x).split(C, dim=2)
-        heads = lambda t: t.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
-        y = F.scaled_dot_product_attention(heads(q), heads(k), heads(v), is_causal=True)
+        q, k, v = self.qkv(x).split([C, self.d_kv, self.d_kv], dim=2)
+        heads = lambda t: t.view(B, T, -1, C // self.n_head).transpose(1, 2)
+        q, k, v = heads(q), heads(k), heads(v)
+        if self.rotary is not None:
+            q, k = self.rotary(q, k)
+        y = F.scaled_dot_product_attention(q, k, v, is_causal=True,
+                                           enable_gqa=self.n_kv_head != self.n_head)
         return self.proj(y.transpose(1, 2).reshape(B, T, C))
 
 
@@ -60,11 +88,17 @@ class _Block(nn.Module):
         self.ln1 = nn.LayerNorm(c.d_model)
         self.attn = _Attention(c)
         self.ln2 = nn.LayerNorm(c.d_model)
-        self.fc = nn.Linear(c.d_model, c.d_ff, bias=False)
-        self.out = nn.Linear(c.d_ff, c.d_model, bias=False)
+        self.ff = None
+        if c.mlp == "gated":
+            self.ff = GatedFeedForward(c.d_model, c.d_ff, c.activation)
+        else:
+            self.fc = nn.Linear(c.d_model, c.d_ff, bias=False)
+            self.out = nn.Linear(c.d_ff, c.d_model, bias=False)
 
     def forward(self, x):
         x = x + self.attn(self.ln1(x))
+        if self.ff is not None:
+            return x + self.ff(self.ln2(x))
         return x + self.out(F.gelu(self.fc(self.ln2(x))))
 
 
@@ -73,7 +107,7 @@ class GPT(nn.Module):
         super().__init__()
         self.c = c
         self.tok = nn.Embedding(c.vocab, c.d_model)
-        self.pos = nn.Embedding(c.seq_len, c.d_model)
+        self.pos = nn.Embedding(c.seq_len, c.d_model) if c.positions == "learned" else None
         self.blocks = nn.ModuleList([_Block(c) for _ in range(c.n_layer)])
         self.ln_f = nn.LayerNorm(c.d_model)
         self.head = nn.Linear(c.d_model, c.vocab, bias=False)
@@ -86,7 +120,9 @@ class GPT(nn.Module):
 
     def forward(self, idx):
         T = idx.shape[1]
-        x = self.tok(idx) + self.pos(torch.arange(T, device=idx.device))
+        x = self.tok(idx)
+        if self.pos is not None:
+            x = x + self.pos(torch.arange(T, device=idx.device))
         for b in self.blocks:
             x = b(x)
         return self.head(self.ln_f(x))

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -84,7 +85,7 @@ class Rotary:
             raise ValueError(f"rotary base must be positive, not {base}")
         self.dim, self.base, self.interleaved, self.scaling = dim, float(base), bool(interleaved), scaling
         self.frequencies, self.magnitude = _frequencies(dim, self.base, scaling)
-        self._turns = (ctypes.c_double * (dim // 2))(*[w / (2 * math.pi) for w in self.frequencies])
+        self._turns = array("d", [w / (2 * math.pi) for w in self.frequencies])
 
     def __call__(self, q, k=None, positions=None):
         """The turned q, or (q, k): new tensors of the same shape, type and order in
@@ -142,7 +143,7 @@ def _run(rotary, inverse, positions, start, dev, tensors):
         a.dtype, a.batch, a.len, a.head_dim = _CODE[x.dtype], x.shape[0], x.shape[2], x.shape[3]
         outs.append(y)
         kept.append(x)
-    a.turns = ctypes.addressof(rotary._turns)
+    a.turns = rotary._turns.buffer_info()[0]
     a.dim, a.interleaved, a.inverse = rotary.dim, rotary.interleaved, inverse
     a.factor, a.start = rotary.magnitude, start
     if positions is not None:

@@ -1,13 +1,15 @@
 """Refusals and host logic of the operators around the optimizer step; no GPU."""
+import copy
 import ctypes
 import math
+import pickle
 from array import array
 
 import pytest
 import torch
 
-from scao_b200 import (Rotary, RotaryScaling, _lib, clip_grad_norm_, clip_grads_with_norm_,
-                       get_total_norm)
+from scao_b200 import (GatedFeedForward, Rotary, RotaryScaling, _lib, clip_grad_norm_,
+                       clip_grads_with_norm_, gated_ff, get_total_norm, gpt)
 from scao_b200.clip import _layout
 
 
@@ -133,6 +135,75 @@ def test_rotary_frequencies():
     assert yarn.frequencies[0] == plain[0] and math.isclose(yarn.frequencies[-1], plain[-1] / 8)
     assert math.isclose(yarn.magnitude, 0.1 * math.log(8) + 1)
     assert all(p / 8 <= y <= p for p, y in zip(plain, yarn.frequencies))
+
+
+def test_rotary_copies_and_pickles():
+    r = Rotary(8, base=500.0, scaling=RotaryScaling("linear", 2.0))
+    for c in (copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert c._turns == r._turns and c.scaling == r.scaling and c.dim == 8
+
+
+# --------------------------------------------------------------- gated_ff
+def test_gated_ff_refusals():
+    b = torch.bfloat16
+    x, w = torch.zeros(3, 8, dtype=b), torch.zeros(5, 8, dtype=b)
+    with pytest.raises(ValueError, match="activation"):
+        gated_ff(x, w, w, activation="relu")
+    with pytest.raises(ValueError, match="activation"):
+        GatedFeedForward(8, 16, "tanh")
+    for args in ((x, w, w[:4]), (x[:, :7], w, w), (x, w[0], w[0]), (x[0, 0], w, w), (x, w[:, :7], w)):
+        with pytest.raises(ValueError, match="must be"):
+            gated_ff(*args)
+    with pytest.raises(ValueError, match="no values"):
+        gated_ff(x, w[:0], w[:0])
+    for args in ((x.float(), w.float(), w.float()), (x, w.half(), w), (x.half(), w, w), (x.double(),) * 3):
+        with pytest.raises((TypeError, ValueError)):
+            gated_ff(*args)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        gated_ff(x, w, w)
+
+
+def test_gated_ff_c_entry_checks():
+    L = _lib.lib()
+    good = dict(x=4096, w_gate=4096, w_up=4096, h=4096, saved=4096, dh=4096, dx=4096, workspace=4096,
+                ldx=8, ldg=8, ldu=8, lddh=5, rows=3, d=8, ff=5, dtype=_lib.BF16, act=0)
+
+    def call(f, **kw):
+        a = _lib.GatedFfArgs()
+        for k, v in {**good, **kw}.items():
+            setattr(a, k, v)
+        return f(ctypes.byref(a), None)
+
+    both = (dict(x=4104), dict(x=None), dict(w_gate=4098), dict(ldx=12), dict(ldg=0), dict(ldu=-8), dict(d=0),
+            dict(ff=0), dict(rows=-1), dict(dtype=0), dict(dtype=3), dict(act=3), dict(act=-1), dict(d=9))
+    for kw in both:
+        assert call(L.scao_gated_ff_forward, **kw) == 1, kw
+        assert call(L.scao_gated_ff_backward, **kw) == 1, kw
+    assert call(L.scao_gated_ff_forward, h=None) == 1
+    assert call(L.scao_gated_ff_forward, rows=0) == 0
+    for kw in (dict(saved=None), dict(dh=None), dict(workspace=None), dict(workspace=4104), dict(dw_gate=4096),
+               dict(dw_up=4096), dict(rows=0)):
+        assert call(L.scao_gated_ff_backward, **kw) == 1, kw
+    assert L.scao_gated_ff_forward(None, None) == 1
+    assert L.scao_gated_ff_saved_bytes(1, 1) == 128 * 128 * 8
+
+
+# ----------------------------------------------------------------- the model
+@pytest.mark.parametrize("kw", [dict(mlp="moe"), dict(positions="none"), dict(n_kv_head=5), dict(n_kv_head=0)])
+def test_gpt_config_refuses(kw):
+    with pytest.raises(ValueError):
+        gpt.GPTConfig(**kw)
+
+
+def test_gpt_shapes():
+    c = gpt.GPTConfig(n_layer=1, d_model=32, n_head=4, d_ff=48, vocab=50, seq_len=8, mlp="gated",
+                      positions="rotary", n_kv_head=2)
+    names = {n: tuple(p.shape) for n, p in gpt.GPT(c).named_parameters()}
+    assert names["blocks.0.attn.qkv.weight"] == (64, 32) and names["blocks.0.ff.gate.weight"] == (48, 32)
+    assert names["blocks.0.ff.out.weight"] == (32, 48) and not any("pos" in n or ".fc" in n for n in names)
+    plain = dict(n_layer=1, d_model=32, n_head=4, d_ff=48, vocab=50, seq_len=8)
+    logits = gpt.GPT(gpt.GPTConfig(**plain))(torch.arange(8)[None])          # the default runs on the CPU
+    assert logits.shape == (1, 8, 50)
 
 
 def test_rotary_c_entry_checks():
