@@ -165,12 +165,12 @@ SIGNATURES = {
     "scao_grad_clip": (C.c_int, [_P, C.c_int, C.c_double, _P, _P]),
     "scao_grad_norm_clip": (C.c_int, [_P, C.c_int, C.c_int, C.c_double, _P, _P, _P]),
     "scao_grads_overlap": (C.c_int, [_P, C.c_int]),
-    "scao_rotary": (C.c_int, [C.POINTER(RotaryArgs), _P]),
+    "scao_rotary": (C.c_int, [_P, _P]),
     "scao_gated_ff_saved_bytes": (C.c_int64, [C.c_int, C.c_int]),
     "scao_gated_ff_workspace_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
     "scao_gated_ff_status_word": (C.POINTER(C.c_int), []),
-    "scao_gated_ff_forward": (C.c_int, [C.POINTER(GatedFfArgs), _P]),
-    "scao_gated_ff_backward": (C.c_int, [C.POINTER(GatedFfArgs), _P]),
+    "scao_gated_ff_forward": (C.c_int, [_P, _P]),
+    "scao_gated_ff_backward": (C.c_int, [_P, _P]),
     "scao_version": (C.c_char_p, []),
     "scao_divc_check": (C.c_int, [_P, _P, C.c_int, _P, _P]),
     "scao_tc_selftest": (C.c_int, [_P, _P, _P, C.c_int, C.c_int, _P, C.c_int, _P]),

@@ -16,7 +16,7 @@ from array import array
 import torch
 
 from . import _lib
-from .cuda import _CODE, _stream
+from .cuda import _CODE, _launch
 
 _KIND = {1.0: 0, 2.0: 1, math.inf: 2}
 
@@ -33,39 +33,55 @@ def _layout(t):
     return dense, False
 
 
-def _table(tensors, write):
-    """(rows of the C table, tensors behind them, [(strided gradient, its packed copy)],
-    device).  Strided gradients that are not dense are packed for the call; tensors
-    that will be written must not share memory."""
-    dev = tensors[0].device
-    rows, kept, packed = [], [], []
+def _refuse(tensors):
+    """Raises for the first tensor that is not a strided one of a supported type on the
+    device of the others."""
     for t in tensors:
         if t.layout != torch.strided:
             raise TypeError(f"unsupported gradient layout {t.layout}")
-        code = _CODE.get(t.dtype)
-        if code is None:
+        if t.dtype not in _CODE:
             raise TypeError(f"unsupported gradient dtype {t.dtype}")
-        if t.device != dev:
-            raise ValueError(f"the gradients must be on one device, not {dev} and {t.device}")
-        if not t.is_contiguous():
+        if t.device != tensors[0].device:
+            raise ValueError("the gradients must be on one device, not "
+                             f"{tensors[0].device} and {t.device}")
+
+
+def _table(tensors, write):
+    """(rows of the C table, tensors behind them, [(strided gradient, its packed copy)],
+    device number).  Strided gradients that are not dense are packed for the call; tensors
+    that will be written must not share memory."""
+    n, index = len(tensors), tensors[0].get_device()
+    codes = [_CODE.get(t.dtype, -1) for t in tensors]
+    get = torch.Tensor
+    if index < 0 or -1 in codes or list(map(get.get_device, tensors)).count(index) != n or \
+            [t.layout for t in tensors].count(torch.strided) != n:
+        _refuse(tensors)
+    packed = []
+    if not all(map(get.is_contiguous, tensors)):
+        tensors = list(tensors)
+        for i, t in enumerate(tensors):
+            if t.is_contiguous():
+                continue
             dense, overlapping = _layout(t)
             if overlapping and write:
                 raise ValueError("a gradient shares memory with itself (an expanded view): "
                                  "it cannot be scaled in place")
             if not dense:
-                packed.append((t, t.contiguous()))
-                t = packed[-1][1]
-        rows += (t.data_ptr(), t.numel(), code)
-        kept.append(t)
+                tensors[i] = t.detach().contiguous()
+                packed.append((t, tensors[i]))
+    rows = [0] * (3 * n)
+    rows[0::3] = list(map(get.data_ptr, tensors))
+    rows[1::3] = list(map(get.numel, tensors))
+    rows[2::3] = codes
     table = array("q", rows)
     if write:
-        rc = _lib.lib().scao_grads_overlap(table.buffer_info()[0], len(tensors))
+        rc = _lib.lib().scao_grads_overlap(table.buffer_info()[0], n)
         if rc == 1:
             raise ValueError("two gradients share memory: each can be scaled only once")
         _lib.check(rc, "scao_grads_overlap")
-    if dev.type != "cuda":
+    if not tensors[0].is_cuda:
         raise RuntimeError("scao_b200: gradients must be CUDA tensors (no CPU path)")
-    return table, kept, packed, dev
+    return table, tensors, packed, index
 
 
 def _kind(norm_type):
@@ -85,7 +101,7 @@ def _max_norm(max_norm):
 def _grads(parameters):
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    return [p.grad for p in parameters if p.grad is not None]
+    return [g for g in [p.grad for p in parameters] if g is not None]
 
 
 def _refuse_nonfinite(total, norm_type):
@@ -95,18 +111,24 @@ def _refuse_nonfinite(total, norm_type):
                            "by it all the same")
 
 
-def _workspace(n, dev):
-    size = int(_lib.lib().scao_grad_norm_workspace_bytes(n))
-    return torch.empty(size, dtype=torch.uint8, device=dev)
+def _outputs(n, index):
+    """(the norm, the workspace) of ``n`` gradients."""
+    dev = torch.device("cuda", index)
+    return (torch.empty((), dtype=torch.float32, device=dev),
+            torch.empty(_lib.lib().scao_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev))
 
 
 def _finish(grads, packed):
+    """What an in-place operation on the gradients ends with."""
     for g, copy in packed:
-        g.copy_(copy)
-    torch.autograd.graph.increment_version([g for g in grads if not g.is_inference()])
+        with torch.no_grad():
+            g.copy_(copy)
+    try:
+        torch.autograd.graph.increment_version(grads)
+    except RuntimeError:            # inference tensors have no version
+        torch.autograd.graph.increment_version([g for g in grads if not g.is_inference()])
 
 
-@torch.no_grad()
 def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False):
     """The norm of all values of ``tensors`` (a tensor or an iterable) as if they were
     one vector: a float32 scalar on their device.  ``norm_type`` is 1, 2 or inf;
@@ -116,19 +138,16 @@ def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False):
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         return torch.tensor(0.0)
-    table, _kept, _, dev = _table(tensors, write=False)
     n = len(tensors)
-    total = torch.empty((), dtype=torch.float32, device=dev)
-    ws = _workspace(n, dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().scao_grad_norm(table.buffer_info()[0], n, kind, ws.data_ptr(),
-                                             total.data_ptr(), _stream(dev)), "scao_grad_norm")
+    table, _kept, _, index = _table(tensors, write=False)
+    total, ws = _outputs(n, index)
+    _launch("scao_grad_norm", index, _lib.lib().scao_grad_norm, table.buffer_info()[0], n, kind,
+            ws.data_ptr(), total.data_ptr())
     if error_if_nonfinite:
         _refuse_nonfinite(total, norm_type)
     return total
 
 
-@torch.no_grad()
 def clip_grads_with_norm_(parameters, max_norm, total_norm):
     """Scales the gradients of ``parameters`` (a tensor or an iterable) in place by
     min(1, max_norm / (total_norm + 1e-6)); ``total_norm`` is a scalar tensor on their
@@ -137,17 +156,15 @@ def clip_grads_with_norm_(parameters, max_norm, total_norm):
     grads = _grads(parameters)
     if not grads or max_norm == math.inf:
         return
-    table, _kept, packed, dev = _table(grads, write=True)
-    if total_norm.numel() != 1 or total_norm.device != dev:
+    table, _kept, packed, index = _table(grads, write=True)
+    if total_norm.numel() != 1 or total_norm.get_device() != index:
         raise ValueError("total_norm must be one number on the gradients' device")
-    total = total_norm.to(torch.float32)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().scao_grad_clip(table.buffer_info()[0], len(grads), max_norm,
-                                             total.data_ptr(), _stream(dev)), "scao_grad_clip")
+    total = total_norm.detach().to(torch.float32)
+    _launch("scao_grad_clip", index, _lib.lib().scao_grad_clip, table.buffer_info()[0], len(grads),
+            max_norm, total.data_ptr())
     _finish(grads, packed)
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Clips the gradients of ``parameters`` (a tensor or an iterable) in place so that
     their norm, taken over all of them as one vector, is at most ``max_norm``:
@@ -162,20 +179,16 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         return torch.tensor(0.0)
     if max_norm == math.inf:
         return get_total_norm(grads, norm_type, error_if_nonfinite)
-    table, _kept, packed, dev = _table(grads, write=True)
-    n = len(grads)
-    total = torch.empty((), dtype=torch.float32, device=dev)
-    ws = _workspace(n, dev)
-    L, at = _lib.lib(), table.buffer_info()[0]
-    with torch.cuda.device(dev):
-        if error_if_nonfinite:
-            _lib.check(L.scao_grad_norm(at, n, kind, ws.data_ptr(), total.data_ptr(), _stream(dev)),
-                       "scao_grad_norm")
-            _refuse_nonfinite(total, norm_type)
-            _lib.check(L.scao_grad_clip(at, n, max_norm, total.data_ptr(), _stream(dev)),
-                       "scao_grad_clip")
-        else:
-            _lib.check(L.scao_grad_norm_clip(at, n, kind, max_norm, ws.data_ptr(), total.data_ptr(),
-                                             _stream(dev)), "scao_grad_norm_clip")
+    n, L = len(grads), _lib.lib()
+    table, _kept, packed, index = _table(grads, write=True)
+    at = table.buffer_info()[0]
+    total, ws = _outputs(n, index)
+    if error_if_nonfinite:
+        _launch("scao_grad_norm", index, L.scao_grad_norm, at, n, kind, ws.data_ptr(), total.data_ptr())
+        _refuse_nonfinite(total, norm_type)
+        _launch("scao_grad_clip", index, L.scao_grad_clip, at, n, max_norm, total.data_ptr())
+    else:
+        _launch("scao_grad_norm_clip", index, L.scao_grad_norm_clip, at, n, kind, max_norm, ws.data_ptr(),
+                total.data_ptr())
     _finish(grads, packed)
     return total

@@ -28,6 +28,19 @@ def _stream(dev):
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+def _launch(what, index, fn, *args):
+    """``fn(*args, stream)`` on device ``index`` and its current stream.  (The raw stream
+    handle and the device number: the stream objects of ``torch.cuda`` cost several
+    microseconds, as much as a small kernel.)"""
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
+
+
 def fused_kronecker_precond(U_l, s_l_inv4, U_r, s_r_inv4, G):
     """out = G + U_l ((s_l s_r^T - 1) o (U_l^T G U_r)) U_r^T, same shape and
     dtype as G (cuda/__init__.py:149-185, formula :78-99)."""

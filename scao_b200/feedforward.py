@@ -13,85 +13,99 @@ copied first.  ``GatedFeedForward`` is the block with its output projection.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 import torch.nn as nn
 
 from . import _lib
-from .cuda import _CODE, _on_cuda, _stream
+from .cuda import _CODE, _launch
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 
+# ScaoGatedFf: ten addresses, four row pitches, six numbers
+_ARGS = struct.Struct("@10P4q6i")
+
+
 def _rows(t):
-    """``t`` (2-D) as the kernels read it: neighbouring values of a row adjacent, rows a
-    multiple of 16 bytes apart, the first on 16 bytes."""
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and \
-            (t.shape[0] == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])):
-        return t
-    n = t.shape[1]
-    p = torch.zeros(t.shape[0], (n + 7) // 8 * 8, dtype=t.dtype, device=t.device)
-    p[:, :n] = t
-    return p[:, :n]
+    """(``t`` (2-D) as the kernels read it: neighbouring values of a row adjacent, rows a
+    multiple of 16 bytes apart, the first on 16 bytes; its address; its row pitch)."""
+    n, p = t.shape[1], t.data_ptr()
+    if p & 15 == 0:
+        if n & 7 == 0 and t.is_contiguous():
+            return t, p, n
+        if t.stride(1) == 1 or n == 1:
+            pitch = t.stride(0) if t.shape[0] > 1 else (n + 7) & ~7
+            if pitch & 7 == 0 and pitch >= n:
+                return t, p, pitch
+    wide = torch.zeros(t.shape[0], (n + 7) & ~7, dtype=t.dtype, device=t.device)
+    wide[:, :n] = t
+    return wide, wide.data_ptr(), wide.shape[1]
 
 
-def _pitch(t):
-    """Row pitch in values; of a single row any that is allowed."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+def _forward(x, w_gate, w_up, act, train):
+    """(h, what the gradient reads or None)."""
+    L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
+    h = torch.empty((rows, ff), dtype=x.dtype, device=x.device)
+    saved = None
+    if train:
+        saved = torch.empty(L.scao_gated_ff_saved_bytes(rows, ff), dtype=torch.uint8, device=x.device)
+    if rows:
+        (x, px, lx), (w_gate, pg, lg), (w_up, pu, lu) = _rows(x), _rows(w_gate), _rows(w_up)
+        args = _ARGS.pack(px, pg, pu, h.data_ptr(), saved.data_ptr() if train else 0, 0, 0, 0, 0, 0,
+                          lx, lg, lu, 0, rows, d, ff, _CODE[x.dtype], act, 0)
+        _launch("scao_gated_ff_forward", x.get_device(), L.scao_gated_ff_forward, args)
+    return h, saved
 
 
-def _args(x, w_gate, w_up, act):
-    a = _lib.GatedFfArgs()
-    a.x, a.w_gate, a.w_up = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
-    a.ldx, a.ldg, a.ldu = _pitch(x), _pitch(w_gate), _pitch(w_up)
-    a.rows, a.d, a.ff, a.dtype, a.act = x.shape[0], x.shape[1], w_gate.shape[0], _CODE[x.dtype], act
-    return a
+def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w):
+    """(dx, dw_gate, dw_up), None where not needed."""
+    L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
+    like = dict(dtype=x.dtype, device=x.device)
+    dx = torch.empty((rows, d), **like) if need_x else None
+    new = torch.empty if rows else torch.zeros
+    dwg, dwu = (new((ff, d), **like), new((ff, d), **like)) if need_w else (None, None)
+    if rows:
+        (x, px, lx), (w_gate, pg, lg), (w_up, pu, lu) = _rows(x), _rows(w_gate), _rows(w_up)
+        if dh.stride(1) != 1:
+            dh = dh.contiguous()
+        ws = torch.empty(L.scao_gated_ff_workspace_bytes(rows, d, ff), dtype=torch.uint8, device=x.device)
+        at = [0 if t is None else t.data_ptr() for t in (dx, dwg, dwu)]
+        args = _ARGS.pack(px, pg, pu, 0, saved.data_ptr(), dh.data_ptr(), *at, ws.data_ptr(),
+                          lx, lg, lu, dh.stride(0), rows, d, ff, _CODE[x.dtype], act, 0)
+        _launch("scao_gated_ff_backward", x.get_device(), L.scao_gated_ff_backward, args)
+    return dx, dwg, dwu
+
+
+class _Once(torch.autograd.Function):
+    """A gradient taken under create_graph: it depends on ``sources``, and asking for
+    that dependence raises instead of passing for a constant."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("gated_ff is differentiable once: its gradient has no gradient")
 
 
 class _GatedFF(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, act, train):
-        dev, L = x.device, _lib.lib()
-        rows, ff = x.shape[0], w_gate.shape[0]
-        h = torch.empty(rows, ff, dtype=x.dtype, device=dev)
-        saved = None
-        if train:
-            saved = torch.empty(int(L.scao_gated_ff_saved_bytes(rows, ff)), dtype=torch.uint8, device=dev)
-        if rows:
-            ins = _rows(x), _rows(w_gate), _rows(w_up)
-            a = _args(*ins, act)
-            a.h, a.saved = h.data_ptr(), saved.data_ptr() if train else None
-            with torch.cuda.device(dev):
-                _lib.check(L.scao_gated_ff_forward(ctypes.byref(a), _stream(dev)), "scao_gated_ff_forward")
-        if train:
-            ctx.act = act
-            ctx.save_for_backward(x, w_gate, w_up, saved)
+    def forward(ctx, x, w_gate, w_up, act):
+        h, saved = _forward(x, w_gate, w_up, act, True)
+        ctx.act = act
+        ctx.save_for_backward(x, w_gate, w_up, saved)
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x, w_gate, w_up, saved = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dev, L = x.device, _lib.lib()
-        rows = x.shape[0]
-        new = torch.empty if rows else torch.zeros
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dwg, dwu = (new(w_gate.shape, dtype=x.dtype, device=dev) if need_w else None for _ in range(2))
-        if rows:
-            ins = _rows(x), _rows(w_gate), _rows(w_up)
-            a = _args(*ins, ctx.act)
-            if dh.stride(1) != 1:
-                dh = dh.contiguous()
-            ws = torch.empty(int(L.scao_gated_ff_workspace_bytes(a.rows, a.d, a.ff)), dtype=torch.uint8,
-                             device=dev)
-            a.dh, a.lddh, a.saved, a.workspace = dh.data_ptr(), dh.stride(0), saved.data_ptr(), ws.data_ptr()
-            a.dx = dx.data_ptr() if need_x else None
-            a.dw_gate, a.dw_up = (dwg.data_ptr(), dwu.data_ptr()) if need_w else (None, None)
-            with torch.cuda.device(dev):
-                _lib.check(L.scao_gated_ff_backward(ctypes.byref(a), _stream(dev)), "scao_gated_ff_backward")
-        return dx, dwg, dwu, None, None
+        need, (x, w_gate, w_up, saved) = ctx.needs_input_grad, ctx.saved_tensors
+        grads = _backward(x, w_gate, w_up, saved, dh.detach(), ctx.act, need[0], need[1] or need[2])
+        if torch.is_grad_enabled():
+            grads = [None if g is None else _Once.apply(g, x, w_gate, w_up, dh) for g in grads]
+        return *grads, None
 
 
 def gated_ff(x, w_gate, w_up, activation="silu"):
@@ -114,10 +128,14 @@ def gated_ff(x, w_gate, w_up, activation="silu"):
                         f"autocast), not {x.dtype}, {w_gate.dtype}, {w_up.dtype}")
     if x.numel() // x.shape[-1] >= 1 << 31 or max(w_gate.shape) >= 1 << 23:
         raise ValueError("gated_ff takes fewer than 2^31 rows and widths below 2^23")
-    _on_cuda(x, w_gate, w_up)
-    train = torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad)
-    h = _GatedFF.apply(x.reshape(-1, x.shape[-1]), w_gate, w_up, act, train)
-    return h.view(*x.shape[:-1], w_gate.shape[0])
+    if not x.is_cuda or w_gate.get_device() != x.get_device() or w_up.get_device() != x.get_device():
+        raise RuntimeError("scao_b200: x, w_gate and w_up must be on one CUDA device (no CPU path)")
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+        h = _GatedFF.apply(flat, w_gate, w_up, act)
+    else:
+        h, _ = _forward(flat, w_gate, w_up, act, False)
+    return h if x.dim() == 2 else h.view(*x.shape[:-1], w_gate.shape[0])
 
 
 class GatedFeedForward(nn.Module):

@@ -14,15 +14,15 @@ CUDA tensors of one device.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from array import array
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from .cuda import _CODE, _on_cuda, _stream
+from .cuda import _CODE, _launch
 
 MAX_DIM = 512
 
@@ -91,15 +91,12 @@ class Rotary:
         """The turned q, or (q, k): new tensors of the same shape, type and order in
         memory.  ``positions``: None counts from 0, an int from there, an integer tensor
         gives each token's, (length) or (batch, length)."""
-        for name, t in (("q", q), ("k", k)):
-            if t is None:
-                continue
-            if t.dim() != 4:
-                raise ValueError(f"{name} must be (batch, heads, length, head_dim), not {tuple(t.shape)}")
-            if t.dtype not in _CODE:
-                raise TypeError(f"unsupported dtype {t.dtype}")
-            if t.shape[3] < self.dim:
-                raise ValueError(f"head_dim {t.shape[3]} is below the rotary dim {self.dim}")
+        if q.dim() != 4 or q.shape[3] < self.dim or (k is not None and k.dim() != 4):
+            raise ValueError("q and k must be (batch, heads, length, head_dim) with at least "
+                             f"{self.dim} values a head, not {tuple(q.shape)}"
+                             + ("" if k is None else f", {tuple(k.shape)}"))
+        if q.dtype not in _CODE:
+            raise TypeError(f"unsupported dtype {q.dtype}")
         if k is not None and (k.dtype != q.dtype or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]):
             raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must share "
                              "batch, length, head_dim and dtype")
@@ -114,45 +111,60 @@ class Rotary:
             start, positions = int(positions), None
             if abs(start) >= 1 << 52:
                 raise ValueError(f"position {start} is out of range")
-        dev = _on_cuda(q, *(t for t in (k, positions) if isinstance(t, torch.Tensor)))
-        out = _Turn.apply(self, False, positions, start, dev, q, k)
-        return out[0] if k is None else out
+        index = q.get_device()
+        if not q.is_cuda or (k is not None and k.get_device() != index) or \
+                (positions is not None and positions.get_device() != index):
+            raise RuntimeError("scao_b200: q, k and positions must be on one CUDA device (no CPU path)")
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            out = _Turn.apply(self, False, positions, start, index, q, k)
+        else:
+            out = _run(self, False, positions, start, index, (q, k))
+        return out[0] if k is None else tuple(out)
+
+
+# ScaoRotary, field by field: two addresses each of the inputs and the results, their
+# strides (batch, head, token of both), turns and positions, the positions' strides and
+# start, heads of both, eight numbers, the factor
+_ARGS = struct.Struct("@4P12q2P3q10ifi")
+_NONE = (0, 0, (0, 0, 0), (0, 0, 0), 0)
 
 
 def _strides(t):
     """Batch, head and token strides; 0 where there is one only."""
-    return [st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride()[:3])]
+    (b, h, n, _), (sb, sh, sn, _) = t.shape, t.stride()
+    return (sb if b > 1 else 0, sh if h > 1 else 0, sn if n > 1 else 0)
 
 
-def _run(rotary, inverse, positions, start, dev, tensors):
+def _run(rotary, inverse, positions, start, index, tensors):
     """The turned tensors (None stays None)."""
-    a = _lib.RotaryArgs()
-    outs, kept = [], []
-    for i, x in enumerate(tensors):
+    outs, kept, parts = [], [], []
+    for x in tensors:
         if x is None:
             outs.append(None)
+            parts.append(_NONE)
             continue
         if x.stride(3) != 1:
             x = x.contiguous()
         y = torch.empty_like(x)
         if y.stride(3) != 1:
-            y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        a.src[i], a.dst[i] = x.data_ptr(), y.data_ptr()
-        a.src_stride[i][:], a.dst_stride[i][:] = _strides(x), _strides(y)
-        a.heads[i] = x.shape[1]
-        a.dtype, a.batch, a.len, a.head_dim = _CODE[x.dtype], x.shape[0], x.shape[2], x.shape[3]
+            y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        parts.append((x.data_ptr(), y.data_ptr(), _strides(x), _strides(y), x.shape[1]))
         outs.append(y)
         kept.append(x)
-    a.turns = rotary._turns.buffer_info()[0]
-    a.dim, a.interleaved, a.inverse = rotary.dim, rotary.interleaved, inverse
-    a.factor, a.start = rotary.magnitude, start
+    if not kept:
+        return outs
+    x = kept[0]
+    at, wide, sb, sn = 0, 0, 0, 0
     if positions is not None:
-        a.positions, a.positions_64 = positions.data_ptr(), positions.dtype == torch.int64
-        a.pos_stride_t = positions.stride(-1) if positions.shape[-1] > 1 else 0
-        a.pos_stride_b = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-    if kept:
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().scao_rotary(ctypes.byref(a), _stream(dev)), "scao_rotary")
+        at, wide = positions.data_ptr(), positions.dtype == torch.int64
+        sn = positions.stride(-1) if positions.shape[-1] > 1 else 0
+        sb = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    (qs, qd, qss, qds, qh), (ks, kd, kss, kds, kh) = parts
+    b, _, n, hd = x.shape
+    args = _ARGS.pack(qs, ks, qd, kd, *qss, *kss, *qds, *kds, rotary._turns.buffer_info()[0], at, sb, sn,
+                      start, qh, kh, _CODE[x.dtype], b, n, hd, rotary.dim, rotary.interleaved, wide, inverse,
+                      rotary.magnitude, 0)
+    _launch("scao_rotary", index, _lib.lib().scao_rotary, args)
     return outs
 
 
@@ -160,19 +172,20 @@ class _Turn(torch.autograd.Function):
     """The rotation, or its transpose (``inverse``), which is its gradient."""
 
     @staticmethod
-    def forward(ctx, rotary, inverse, positions, start, dev, q, k):
-        ctx.args = rotary, inverse, start, dev
+    def forward(ctx, rotary, inverse, positions, start, index, q, k):
+        ctx.args = rotary, inverse, start, index
         ctx.save_for_backward(positions)
         ctx.set_materialize_grads(False)
-        return tuple(_run(rotary, inverse, positions, start, dev, (q, k)))
+        return tuple(_run(rotary, inverse, positions, start, index, (q, k)))
 
     @staticmethod
     def backward(ctx, gq, gk):
-        rotary, inverse, start, dev = ctx.args
+        rotary, inverse, start, index = ctx.args
         (positions,) = ctx.saved_tensors
-        if not ctx.needs_input_grad[5]:
-            gq = None
-        if not ctx.needs_input_grad[6]:
-            gk = None
-        gq, gk = _Turn.apply(rotary, not inverse, positions, start, dev, gq, gk)
+        need = ctx.needs_input_grad
+        gq, gk = gq if need[5] else None, gk if need[6] else None
+        if torch.is_grad_enabled():                         # differentiable again
+            gq, gk = _Turn.apply(rotary, not inverse, positions, start, index, gq, gk)
+        else:
+            gq, gk = _run(rotary, not inverse, positions, start, index, (gq, gk))
         return None, None, None, None, None, gq, gk

@@ -225,6 +225,16 @@ def test_gradient_against_differences():
             assert abs(g.reshape(-1)[i].item() - diff) <= tol, (k, i)
 
 
+def test_second_derivative_is_refused():
+    ins = [v.requires_grad_() for v in inputs(9, 64, 40, torch.bfloat16)]
+    dh = randn(9, 40, seed=2)
+    plain = torch.autograd.grad(gated_ff(*ins), ins, dh)
+    graph = torch.autograd.grad(gated_ff(*ins), ins, dh, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, graph))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(graph[0].float().sum(), ins)
+
+
 def test_empty_rows():
     _, wg, wu = inputs(1, 64, 40, torch.bfloat16)
     for shape in ((0, 64), (2, 0, 64)):

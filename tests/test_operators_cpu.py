@@ -227,3 +227,15 @@ def test_rotary_c_entry_checks():
         assert call(**kw) == 1, kw
     assert call(batch=0) == 0
     assert L.scao_rotary(None, None) == 1
+
+
+def test_packed_arguments_match_the_structs():
+    """The packed forms that the calls pass have the fields of the C structs."""
+    from scao_b200 import feedforward, rotary
+    assert rotary._ARGS.size == ctypes.sizeof(_lib.RotaryArgs)
+    assert feedforward._ARGS.size == ctypes.sizeof(_lib.GatedFfArgs)
+    a = _lib.GatedFfArgs.from_buffer_copy(feedforward._ARGS.pack(*range(1, 21)))
+    assert [getattr(a, n) for n, _ in a._fields_] == list(range(1, 21))
+    b = _lib.RotaryArgs.from_buffer_copy(rotary._ARGS.pack(*range(1, 34)))
+    assert [b.src[0], b.dst[1], b.src_stride[1][0], b.dst_stride[1][2], b.turns, b.positions, b.pos_stride_b,
+            b.start, b.heads[1], b.dtype, b.inverse, b.factor] == [1, 4, 8, 16, 17, 18, 19, 21, 23, 24, 31, 32]
