@@ -53,7 +53,7 @@ struct FfGemm {
     int rows, cols;                         // of one result
     int mt, nt, parts;                      // row and column tiles; results (dW: 2)
     int ksteps, segs;                       // 64-deep steps of one segment; segments (dx: 2)
-    int dtype, act, tma_out;
+    int dtype, tma_out;
 };
 
 struct FfTile { int part, m, n; };          // result, row tile, column tile
@@ -77,20 +77,22 @@ SCAO_DEV float ff_sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
 constexpr float TANH_A = 0.7978845608028654f, TANH_B = 0.044715f;   // sqrt(2 / pi)
 
-SCAO_DEV float ff_act(float g, int act) {
-    if (act == SCAO_ACT_SILU) return g * ff_sigmoid(g);
-    if (act == SCAO_ACT_GELU) return g * normcdff(g);
+template <int ACT>
+SCAO_DEV float ff_act(float g) {
+    if (ACT == SCAO_ACT_SILU) return g * ff_sigmoid(g);
+    if (ACT == SCAO_ACT_GELU) return g * normcdff(g);
     // 0.5 (1 + tanh y) = sigmoid(2 y)
     return g * ff_sigmoid(2.f * TANH_A * (g + TANH_B * g * g * g));
 }
 
 // act(g) and act'(g)
-SCAO_DEV void ff_act_grad(float g, int act, float& a, float& d) {
-    if (act == SCAO_ACT_SILU) {
+template <int ACT>
+SCAO_DEV void ff_act_grad(float g, float& a, float& d) {
+    if (ACT == SCAO_ACT_SILU) {
         const float s = ff_sigmoid(g);
         a = g * s;
         d = s * (1.f + g * (1.f - s));
-    } else if (act == SCAO_ACT_GELU) {
+    } else if (ACT == SCAO_ACT_GELU) {
         const float s = normcdff(g);
         a = g * s;
         d = s + g * 0.3989422804014327f * __expf(-0.5f * g * g);
@@ -152,7 +154,7 @@ SCAO_DEV void ff_store_block(const FfGemm& G, int part, const uint32_t* v, unsig
 // accumulators).  Every wait is bounded; when one runs out the CTA records it in
 // *status, issues no more, waits for its copies in flight and both CTAs still meet
 // at the end.
-template <int MODE>
+template <int MODE, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FTHREADS, 1)
 ff_gemm_kernel(const __grid_constant__ FfGemm G) {
     extern __shared__ unsigned char raw[];
@@ -275,24 +277,32 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
             const uint32_t tb = tmem + acc * FN + ((uint32_t)(q * 32) << 16);
             if (MODE == FF_FORWARD) {
                 const int c0 = w.n * 128 + h * 64, cb = (G.cols + 127) >> 7;
-                uint32_t out[32];
+                uint32_t out[32], gr[2][16], ur[2][16];
+                tc_ld16_async(tb + h * 64, gr[0]);
+                tc_ld16_async(tb + 128 + h * 64, ur[0]);
 #pragma unroll
-                for (int c = 0; c < 64; c += 16) {
-                    float g[16], u[16];
-                    tc_ld16(tb + h * 64 + c, g);
-                    tc_ld16(tb + 128 + h * 64 + c, u);
+                for (int c = 0; c < 64; c += 16) {      // the next 16 columns are on their way
+                    uint32_t *g = gr[(c >> 4) & 1], *u = ur[(c >> 4) & 1];
+                    tc_ld16_wait(g);
+                    tc_ld16_wait(u);
+                    if (c + 16 < 64) {
+                        tc_ld16_async(tb + h * 64 + c + 16, gr[((c >> 4) + 1) & 1]);
+                        tc_ld16_async(tb + 128 + h * 64 + c + 16, ur[((c >> 4) + 1) & 1]);
+                    }
                     if (G.saved && row < G.rows && c0 + c < G.cols) {
                         float* p = G.saved + saved_off(row, c0 + c, cb);
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
-                            *(float4*)(p + i * 128) = make_float4(g[i], g[i + 1], g[i + 2], g[i + 3]);
-                            *(float4*)(p + SAVED_U + i * 128) = make_float4(u[i], u[i + 1], u[i + 2], u[i + 3]);
+                            *(uint4*)(p + i * 128) = make_uint4(g[i], g[i + 1], g[i + 2], g[i + 3]);
+                            *(uint4*)(p + SAVED_U + i * 128) = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
                         }
                     }
+                    float y[16];
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2)
-                        out[(c + i) / 2] = pack2(ff_act(g[i], G.act) * u[i], ff_act(g[i + 1], G.act) * u[i + 1],
-                                                 G.dtype);
+                    for (int i = 0; i < 16; ++i)
+                        y[i] = ff_act<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) out[(c + i) / 2] = pack2(y[i], y[i + 1], G.dtype);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -334,40 +344,148 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
 // runs of 64 bytes and more of every array.  HBM bound (14 bytes a value).
 constexpr int PT = 256;
 
+template <int ACT>
 __global__ void __launch_bounds__(PT)
 ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict__ dh, int64_t lddh,
                     uint16_t* __restrict__ dg, uint16_t* __restrict__ du, int64_t ldg, int rows,
-                    int cols, int dtype, int act, int vec) {
+                    int cols, int dtype, int vec) {
     const int cb = (cols + 127) >> 7, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.y * 128 + (warp & 3) * 32 + (lane & 7) * 4;
     if (c >= cols) return;
     const int r0 = blockIdx.x * 128 + (warp >> 2) * 64 + (lane >> 3);
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
-        const int r = r0 + 4 * i;
-        if (r >= rows) break;
-        const float* p = saved + saved_off(r, c, cb);
-        const float4 g = *(const float4*)p, u = *(const float4*)(p + SAVED_U);
-        const uint16_t* d = dh + r * lddh + c;
-        float4 y;
-        if (vec) {
-            y = load4_dt(d, 0, dtype);
-        } else {
-            y.x = load_dt(d, 0, dtype);
-            y.y = c + 1 < cols ? load_dt(d, 1, dtype) : 0.f;
-            y.z = c + 2 < cols ? load_dt(d, 2, dtype) : 0.f;
-            y.w = c + 3 < cols ? load_dt(d, 3, dtype) : 0.f;
+#pragma unroll 1
+    for (int i = 0; i < 16; i += 4) {
+        if (r0 + 4 * i >= rows) break;
+        float4 g[4], u[4], y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                   // all loads first
+            const int r = min(r0 + 4 * (i + k), rows - 1);
+            const float* p = saved + saved_off(r, c, cb);
+            g[k] = ldg_stream4(p);
+            u[k] = ldg_stream4(p + SAVED_U);
+            const uint16_t* d = dh + r * lddh + c;
+            if (vec) {
+                y[k] = load4_dt(d, 0, dtype);
+            } else {
+                y[k].x = load_dt(d, 0, dtype);
+                y[k].y = c + 1 < cols ? load_dt(d, 1, dtype) : 0.f;
+                y[k].z = c + 2 < cols ? load_dt(d, 2, dtype) : 0.f;
+                y[k].w = c + 3 < cols ? load_dt(d, 3, dtype) : 0.f;
+            }
         }
-        float4 a, b;
-        ff_act_grad(g.x, act, a.x, b.x);
-        ff_act_grad(g.y, act, a.y, b.y);
-        ff_act_grad(g.z, act, a.z, b.z);
-        ff_act_grad(g.w, act, a.w, b.w);
-        // the pitch of dg and du is a multiple of 8: the last group may write past
-        // `cols` within it, where the products read nothing
-        store4_dt(du + r * ldg + c, 0, dtype, make_float4(y.x * a.x, y.y * a.y, y.z * a.z, y.w * a.w));
-        store4_dt(dg + r * ldg + c, 0, dtype,
-                  make_float4(y.x * u.x * b.x, y.y * u.y * b.y, y.z * u.z * b.z, y.w * u.w * b.w));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = r0 + 4 * (i + k);
+            if (r >= rows) break;
+            float4 a, b;
+            ff_act_grad<ACT>(g[k].x, a.x, b.x);
+            ff_act_grad<ACT>(g[k].y, a.y, b.y);
+            ff_act_grad<ACT>(g[k].z, a.z, b.z);
+            ff_act_grad<ACT>(g[k].w, a.w, b.w);
+            const float4 d = y[k];
+            // the pitch of dg and du is a multiple of 8: the last group may write past
+            // `cols` within it, where the products read nothing
+            store4_dt(du + r * ldg + c, 0, dtype, make_float4(d.x * a.x, d.y * a.y, d.z * a.z, d.w * a.w));
+            store4_dt(dg + r * ldg + c, 0, dtype,
+                      make_float4(d.x * u[k].x * b.x, d.y * u[k].y * b.y, d.z * u[k].z * b.z,
+                                  d.w * u[k].w * b.w));
+        }
+    }
+}
+
+// Few rows (at most SK_ROWS): the time is one reading of the weights, so no tile
+// waits for a whole operand block.  A warp takes 8 inner columns: the 16 rows of an
+// mma.m16n8k16 A operand are their 8 gate and 8 up weight rows, loaded straight
+// from global memory into the registers that the instruction reads (a contraction
+// may take its terms in any order, so a lane's 16 consecutive bytes serve as the
+// k places of two instructions, in x as in the weights).  Gate and up of one place
+// meet in one thread.  The block's warps share a row's contraction and join in
+// shared memory in a fixed order.
+constexpr int SK_WARPS = 8;
+constexpr int SK_ROWS = 32;
+
+SCAO_DEV void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                        uint32_t b1, bool bf16) {
+    if (bf16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// the 8 values from p on, those beyond the row's end as zeros
+SCAO_DEV uint4 load8_guard(const uint16_t* p, int left) {
+    if (left >= 8) return *(const uint4*)p;
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = 0; i < left; ++i) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int ACT, bool BF16, int NT>
+__global__ void __launch_bounds__(32 * SK_WARPS)
+ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ wg, int64_t ldg,
+                 const uint16_t* __restrict__ wu, int64_t ldu, uint16_t* __restrict__ h, int rows, int d,
+                 int ff) {
+    constexpr int U = NT == 1 ? 4 : 2;          // 32-deep steps in flight
+    __shared__ float part[SK_WARPS][NT * 4][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int f = blockIdx.x * 8 + g;
+    const bool has = f < ff;
+    const uint16_t* pg = wg + (int64_t)min(f, ff - 1) * ldg;
+    const uint16_t* pu = wu + (int64_t)min(f, ff - 1) * ldu;
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+    for (int k0 = warp * 32 * U; k0 < d; k0 += SK_WARPS * 32 * U) {
+        uint4 a[U], b[U], v[NT][U];
+#pragma unroll
+        for (int s = 0; s < U; ++s) {
+            const int k = k0 + 32 * s + 8 * t;
+            a[s] = load8_guard(pg + k, d - k);
+            b[s] = load8_guard(pu + k, d - k);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int r = n * 8 + g;
+                v[n][s] = load8_guard(x + (int64_t)min(r, rows - 1) * ldx + k, r < rows ? d - k : 0);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < U; ++s)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma_16816(acc[n], a[s].x, b[s].x, a[s].y, b[s].y, v[n][s].x, v[n][s].y, BF16);
+                mma_16816(acc[n], a[s].z, b[s].z, a[s].w, b[s].w, v[n][s].z, v[n][s].w, BF16);
+            }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[warp][n * 4 + i][lane] = acc[n][i];
+    __syncthreads();
+    // thread (n, j): columns 2t + j of row group n, gate in place j and up in 2 + j
+    if (warp < NT) {
+        const int n = warp;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float gate = 0.f, upv = 0.f;
+#pragma unroll
+            for (int w = 0; w < SK_WARPS; ++w) {
+                gate += part[w][n * 4 + j][lane];
+                upv += part[w][n * 4 + 2 + j][lane];
+            }
+            const int r = n * 8 + 2 * t + j;
+            if (has && r < rows) {
+                const float y = ff_act<ACT>(gate) * upv;
+                h[(int64_t)r * ff + f] = BF16 ? f_to_bf16_bits(y) : f_to_f16_bits(y);
+            }
+        }
     }
 }
 
@@ -379,17 +497,17 @@ bool map2d(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t
     return scao_tensor_map_2d(m, dtype, base, rows, cols, ld, bx, by);
 }
 
-template <int MODE>
+template <int MODE, int ACT = 0>
 int launch_gemm(FfGemm& G, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.first() && cudaFuncSetAttribute(ff_gemm_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)FSMEM) != cudaSuccess)
+    if (once.first() && cudaFuncSetAttribute(ff_gemm_kernel<MODE, ACT>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FSMEM) != cudaSuccess)
         return SCAO_ERR_LAUNCH;
     const int64_t tiles = (int64_t)G.parts * G.mt * G.nt;
     if (tiles > (1 << 30)) return SCAO_ERR_ARG;
     const int pairs = scao_sm_count() / 2;
     ProfScope p(SLOT_GATED_FF, st);
-    ff_gemm_kernel<MODE><<<2 * (int)(tiles < pairs ? tiles : pairs), FTHREADS, FSMEM, st>>>(G);
+    ff_gemm_kernel<MODE, ACT><<<2 * (int)(tiles < pairs ? tiles : pairs), FTHREADS, FSMEM, st>>>(G);
     SCAO_CHECK_LAUNCH();
     return SCAO_OK;
 }
@@ -419,6 +537,24 @@ int take_status() {
     int* w = status_word();
     if (!w) return SCAO_ERR_LAUNCH;
     return __atomic_exchange_n(w, 0, __ATOMIC_RELAXED) ? SCAO_ERR_TIMEOUT : SCAO_OK;
+}
+
+template <int ACT, bool BF16>
+int launch_skinny(const ScaoGatedFf* f, cudaStream_t st) {
+    const int nt = (f->rows + 7) / 8;
+    auto* kernel = nt == 1 ? ff_skinny_kernel<ACT, BF16, 1>
+                   : nt == 2 ? ff_skinny_kernel<ACT, BF16, 2> : ff_skinny_kernel<ACT, BF16, 4>;
+    ProfScope p(SLOT_GATED_FF, st);
+    kernel<<<(f->ff + 7) / 8, 32 * SK_WARPS, 0, st>>>(
+        (const uint16_t*)f->x, f->ldx, (const uint16_t*)f->w_gate, f->ldg, (const uint16_t*)f->w_up, f->ldu,
+        (uint16_t*)f->h, f->rows, f->d, f->ff);
+    SCAO_CHECK_LAUNCH();
+    return SCAO_OK;
+}
+
+template <int ACT>
+int launch_skinny(const ScaoGatedFf* f, cudaStream_t st) {
+    return f->dtype == SCAO_BF16 ? launch_skinny<ACT, true>(f, st) : launch_skinny<ACT, false>(f, st);
 }
 
 bool aligned(const void* p, int64_t ld) { return p && ((uintptr_t)p & 15) == 0 && ld > 0 && (ld & 7) == 0; }
@@ -452,6 +588,12 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     if (f->rows == 0) return SCAO_OK;
     if (!f->h) return SCAO_ERR_ARG;
     if (int rc = take_status()) return rc;
+    if (!f->saved && f->rows <= SK_ROWS) {
+        const cudaStream_t st = (cudaStream_t)stream;
+        if (f->act == SCAO_ACT_SILU) return launch_skinny<SCAO_ACT_SILU>(f, st);
+        if (f->act == SCAO_ACT_GELU) return launch_skinny<SCAO_ACT_GELU>(f, st);
+        return launch_skinny<SCAO_ACT_GELU_TANH>(f, st);
+    }
     FfGemm G;
     memset(&G, 0, sizeof(G));
     G.tma_out = aligned(f->h, f->ff);
@@ -471,8 +613,10 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     G.parts = G.segs = 1;
     G.ksteps = up(f->d, 64);
     G.dtype = f->dtype;
-    G.act = f->act;
-    return launch_gemm<FF_FORWARD>(G, (cudaStream_t)stream);
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (f->act == SCAO_ACT_SILU) return launch_gemm<FF_FORWARD, SCAO_ACT_SILU>(G, st);
+    if (f->act == SCAO_ACT_GELU) return launch_gemm<FF_FORWARD, SCAO_ACT_GELU>(G, st);
+    return launch_gemm<FF_FORWARD, SCAO_ACT_GELU_TANH>(G, st);
 }
 
 extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
@@ -487,9 +631,11 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
         const int vec = ((uintptr_t)f->dh & 7) == 0 && (f->lddh & 3) == 0 && (f->ff & 3) == 0;
         if (up(f->ff, 128) > 65535) return SCAO_ERR_ARG;
         ProfScope p(SLOT_GATED_FF, st);
-        ff_pointwise_kernel<<<dim3(up(f->rows, 128), up(f->ff, 128)), PT, 0, st>>>(
-            (const float*)f->saved, (const uint16_t*)f->dh, f->lddh, dg, du, ld, f->rows, f->ff, f->dtype,
-            f->act, vec);
+        auto* kernel = f->act == SCAO_ACT_SILU   ? ff_pointwise_kernel<SCAO_ACT_SILU>
+                       : f->act == SCAO_ACT_GELU ? ff_pointwise_kernel<SCAO_ACT_GELU>
+                                                 : ff_pointwise_kernel<SCAO_ACT_GELU_TANH>;
+        kernel<<<dim3(up(f->rows, 128), up(f->ff, 128)), PT, 0, st>>>(
+            (const float*)f->saved, (const uint16_t*)f->dh, f->lddh, dg, du, ld, f->rows, f->ff, f->dtype, vec);
         SCAO_CHECK_LAUNCH();
     }
     FfGemm G;
