@@ -23,6 +23,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "prof.cuh"
@@ -31,47 +32,86 @@
 
 namespace {
 
-enum { FF_FORWARD = 0, FF_DX, FF_DW };
+enum { FF_FORWARD = 0, FF_DX, FF_DW };      // what a work item computes
 
-constexpr int FN = 256;                     // accumulator columns of a tile
 constexpr int FST = 6;                      // pipeline stages
-constexpr uint32_t FOPB = 128 * 64 * 2;     // one 128 x 64 operand block, 16 KB
+constexpr uint32_t FOPB = 128 * 64 * 2;     // one 128 x 64 operand block, 16 KB: two TMA boxes of 64 x 64
 constexpr uint32_t FSTAGE = 2 * FOPB;
 constexpr int FEPI_WARPS = 8;
 constexpr uint32_t FOUTB = 32 * 64 * 2;     // a warp's 32 x 64 block of the result, 4 KB
 constexpr int FTHREADS = 64 + 32 * FEPI_WARPS;
-constexpr int FBAND = 16;                   // row blocks per band of the tile order
+constexpr int FBAND = 16;                   // row tiles per band of the tile order
 constexpr size_t FSMEM = 1024 + (size_t)FST * FSTAGE + FEPI_WARPS * FOUTB;
 static_assert(FSMEM <= 231 * 1024, "shared memory");
 
-struct FfGemm {
-    CUtensorMap a[2], b[2], out[2];
-    void* outp[2];                          // the results, for the stores without TMA
-    float* saved;                           // forward: g and u for the gradient, or null
-    int* status;
-    int64_t ldo;                            // row pitch of the results (values)
-    int rows, cols;                         // of one result
-    int mt, nt, parts;                      // row and column tiles; results (dW: 2)
-    int ksteps, segs;                       // 64-deep steps of one segment; segments (dx: 2)
-    int dtype, tma_out;
+// One product: `parts` results of rows x cols in mt x nt tiles, each the sum over
+// `steps` 64-deep blocks, which `splits` items share.
+struct FfWork {
+    int mode, parts, mt, nt, splits, steps, rows, cols, tma_out;
+    int count0;                             // split: this product's first counter,
+    int64_t partial0;                       // and the first of its partial sums
+    int64_t ldo;
+    void* outp[2];
 };
 
-struct FfTile { int part, m, n; };          // result, row tile, column tile
+struct FfGemm {
+    // boxes 64 wide: 128 rows of what is read K-major (64 of the weights for single CTAs),
+    // 64 of what is read MN-major, 32 of the results (h, or dx, dWg, dWu)
+    CUtensorMap x, w[2], dguk[2], dgum[2], out[3];
+    FfWork work[2];                         // in the order in which a CTA (pair) takes them
+    float* saved;                           // forward: g and u for the gradient, or null
+    float* partial;                         // split tiles: sums of the items
+    int* count;                             // split tiles: items done, per epilogue warp
+    int* status;
+    int extra;                              // see ff_item
+    int dtype;
+};
 
-// tiles in bands of FBAND row blocks, row blocks fastest: the tiles that run at
-// one time share few operand panels, which stay in L2
-__device__ __forceinline__ FfTile ff_tile(const FfGemm& G, int T) {
-    FfTile w;
-    const int per = G.mt * G.nt;
-    w.part = T / per;
-    int t = T - w.part * per;
-    const int band = t / (FBAND * G.nt);
-    t -= band * FBAND * G.nt;
-    const int h = min(FBAND, G.mt - band * FBAND);
-    w.n = t / h;
-    w.m = band * FBAND + t - w.n * h;
-    return w;
+struct FfItem { int w, part, m, n, split, tile; };
+
+// The n-th item of group g of G (a CTA or a pair): items of work[0] in turn, then those
+// of work[1].  Where the first do not come out even, the groups that got one less
+// take `extra` items of the second first: about as many as take the same time.
+SCAO_DEV bool ff_item(const FfGemm& P, int g, int G, int n, FfItem& it) {
+    const FfWork &a = P.work[0], &b = P.work[1];
+    const int na = a.parts * a.mt * a.nt * a.splits, nb = b.parts * b.mt * b.nt * b.splits;
+    const int mine = g < na ? (na - g + G - 1) / G : 0, r = na % G;
+    int i;
+    if (n < mine) {
+        it.w = 0;
+        i = g + n * G;
+    } else {
+        it.w = 1;
+        n -= mine;
+        const int late = r ? G - r : 0, early = min(late * P.extra, nb);
+        if (late && g >= r) {
+            i = g - r + n * late;
+            if (n < P.extra && i < early) goto found;
+            n -= P.extra;
+            if (n < 0) return false;
+        }
+        i = early + g + n * G;
+        if (i >= nb) return false;
+    }
+found:
+    const FfWork& w = P.work[it.w];
+    it.tile = i / w.splits;
+    it.split = i - it.tile * w.splits;
+    const int per = w.mt * w.nt;
+    it.part = it.tile / per;
+    int t = it.tile - it.part * per;
+    // in bands of FBAND row tiles, row tiles fastest: the tiles that run at one time
+    // share few operand panels, which stay in L2
+    const int band = t / (FBAND * w.nt);
+    t -= band * FBAND * w.nt;
+    const int h = min(FBAND, w.mt - band * FBAND);
+    it.n = t / h;
+    it.m = band * FBAND + t - it.n * h;
+    return true;
 }
+
+// first step of a split
+SCAO_DEV int ff_first(const FfWork& w, int split) { return (int)((int64_t)split * w.steps / w.splits); }
 
 SCAO_DEV float ff_sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
@@ -121,97 +161,119 @@ SCAO_DEV void ff_fail(int* status) { *(volatile int*)status = 2; }
 
 // One warp's 32 x 64 block of a result, 16-bit values in `v` (32 pairs of this
 // thread's row): through shared memory, then a TMA store or guarded stores.
-SCAO_DEV void ff_store_block(const FfGemm& G, int part, const uint32_t* v, unsigned char* stage,
-                             int row0, int col0, int lane) {
+SCAO_DEV void ff_store_block(const FfWork& w, const CUtensorMap* map, int part, const uint32_t* v,
+                             unsigned char* stage, int row0, int col0, int lane) {
     if (lane == 0) bulk_wait_read0();
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < 8; ++c)
         *(uint4*)(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) =
             make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-    if (G.tma_out) {
+    if (w.tma_out) {
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-            if (row0 < G.rows && col0 < G.cols) tma_store_2d(&G.out[part], col0, row0, smem_u32(stage));
+            if (row0 < w.rows && col0 < w.cols) tma_store_2d(map, col0, row0, smem_u32(stage));
             bulk_commit();
         }
         return;
     }
     __syncwarp();
-    for (int r = 0; r < 32 && row0 + r < G.rows; ++r) {
-        uint16_t* dst = (uint16_t*)G.outp[part] + (int64_t)(row0 + r) * G.ldo;
+    for (int r = 0; r < 32 && row0 + r < w.rows; ++r) {
+        uint16_t* dst = (uint16_t*)w.outp[part] + (int64_t)(row0 + r) * w.ldo;
 #pragma unroll
         for (int c = lane; c < 64; c += 32)
-            if (col0 + c < G.cols)
+            if (col0 + c < w.cols)
                 dst[col0 + c] = *(const uint16_t*)(stage + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2);
     }
     __syncwarp();
 }
 
-// Roles per CTA: warp 0 TMA producer; warp 1 TMEM owner and (first CTA of the pair)
-// MMA issuer; warps 2-9 epilogue, which overlaps the next tile's main loop (two
+// One tcgen05 product kernel: a CTA (128 x 128 tiles) or, PAIR, the two CTAs of a
+// cluster (256 x 256 tiles, tcgen05.mma.cta_group::2, each CTA staging 128 rows of A
+// and 128 of B).  Roles per CTA: warp 0 TMA producer; warp 1 TMEM owner and (first CTA)
+// MMA issuer; warps 2-9 epilogue, which overlaps the next item's main loop (two
 // accumulators).  Every wait is bounded; when one runs out the CTA records it in
-// *status, issues no more, waits for its copies in flight and both CTAs still meet
-// at the end.
-template <int MODE, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FTHREADS, 1)
+// *status, issues no more, waits for its copies in flight, and both CTAs still meet at
+// the end.
+template <bool PAIR, bool FORWARD, int ACT>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(FTHREADS, 1)
 ff_gemm_kernel(const __grid_constant__ FfGemm G) {
+    constexpr int NC = PAIR ? 2 : 1, TM = 128 * NC, TN = 128 * NC;
+    // the forward tile of one CTA has 64 columns: four warps read it
+    constexpr int EPI = FORWARD && !PAIR ? 4 : FEPI_WARPS;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = (unsigned char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[FST], empty[FST], accf[2], acce[2], fin;
     __shared__ uint32_t tslot;
     __shared__ volatile int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = cluster_ctarank();
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0;
     const bool leader = rank == 0;
+    auto sync_all = [] { if (PAIR) cluster_sync_all(); else __syncthreads(); };
+    auto commit = [](uint64_t* bar) { if (PAIR) tc_commit_pair(bar, 0x3); else tc_commit(bar); };
     if (tid == 0) {
-        for (int i = 0; i < FST; ++i) { mbar_init(&full[i], 2); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&accf[i], 1); mbar_init(&acce[i], 2 * FEPI_WARPS); }
+        for (int i = 0; i < FST; ++i) { mbar_init(&full[i], NC); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&accf[i], 1); mbar_init(&acce[i], NC * EPI); }
         mbar_init(&fin, 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tc_alloc_pair(&tslot, 2 * FN);
+    if (warp == 1) { if (PAIR) tc_alloc_pair(&tslot, 2 * TN); else tc_alloc(&tslot, 2 * TN); }
     tc_fence_before();
-    cluster_sync_all();
+    sync_all();
     tc_fence_after();
     const uint32_t tmem = tslot;
-    const int total = G.parts * G.mt * G.nt;
-    const int cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
-    const int steps = G.ksteps * G.segs;
+    const int grp = blockIdx.x / NC, ngrp = gridDim.x / NC;
+    FfItem it;
     if (warp == 0) {
         if (lane == 0) {
             int stage = 0;
             uint32_t ph = 0, issued = 0, last_ph = 0;
-            for (int T = cid; T < total && !abort_flag; T += ncl) {
-                const FfTile w = ff_tile(G, T);
-                const int i0 = w.m * 256 + 128 * (int)rank;
-                const int j0 = MODE == FF_FORWARD ? w.n * 128 : w.n * FN + 128 * (int)rank;
-                for (int s = 0; s < steps; ++s) {
-                    if (!mbar_wait(&empty[stage], ph ^ 1)) { abort_flag = 1; ff_fail(G.status); break; }
-                    const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
-                    mbar_arrive_expect_tx_cl(fb, FSTAGE);
-                    const uint32_t a = smem_u32(sm + (size_t)stage * FSTAGE), b = a + FOPB;
-                    if (MODE == FF_FORWARD) {
-                        tma_load_2d_pair(a, &G.a[0], s * 64, i0, fb);
-                        tma_load_2d_pair(b, &G.b[rank], s * 64, j0, fb);
-                    } else if (MODE == FF_DX) {
-                        const int g = s >= G.ksteps, k0 = (s - g * G.ksteps) * 64;
-                        tma_load_2d_pair(a, &G.a[g], k0, i0, fb);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            tma_load_2d_pair(b + h * (FOPB / 2), &G.b[g], j0 + 64 * h, k0, fb);
-                    } else {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            tma_load_2d_pair(a + h * (FOPB / 2), &G.a[w.part], i0 + 64 * h, s * 64, fb);
-                            tma_load_2d_pair(b + h * (FOPB / 2), &G.b[0], j0 + 64 * h, s * 64, fb);
-                        }
+            for (int n = 0; !abort_flag && ff_item(G, grp, ngrp, n, it); ++n) {
+                const FfWork& w = G.work[it.w];
+                const int i0 = it.m * TM + 128 * (int)rank;
+                const int j0 = FORWARD ? it.n * (TN / 2) : it.n * TN + 128 * (int)rank;
+                const int s0 = ff_first(w, it.split), s1 = ff_first(w, it.split + 1), half = w.steps >> 1;
+                // one step: waits for its stage, announces its bytes and lets `fill` copy them
+                auto run = [&](auto&& fill) {
+                    for (int s = s0; s < s1; ++s) {
+                        if (!mbar_wait(&empty[stage], ph ^ 1)) { abort_flag = 1; ff_fail(G.status); return; }
+                        const uint32_t bar = PAIR ? mapa_shared(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
+                        if (PAIR) mbar_arrive_expect_tx_cl(bar, FSTAGE); else mbar_expect_tx(&full[stage], FSTAGE);
+                        const uint32_t a = smem_u32(sm) + stage * FSTAGE;
+                        fill(s, a, a + FOPB, [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+                            if (PAIR) tma_load_2d_pair(dst, map, x, y, bar);
+                            else tma_load_2d(dst, map, x, y, &full[stage]);
+                        });
+                        issued |= 1u << stage;
+                        last_ph = (last_ph & ~(1u << stage)) | (ph << stage);
+                        if (++stage == FST) { stage = 0; ph ^= 1; }
                     }
-                    issued |= 1u << stage;
-                    last_ph = (last_ph & ~(1u << stage)) | (ph << stage);
-                    if (++stage == FST) { stage = 0; ph ^= 1; }
+                };
+                constexpr uint32_t HB = FOPB / 2;
+                if (FORWARD) {
+                    const CUtensorMap* wm = &G.w[rank];
+                    run([&](int s, uint32_t a, uint32_t b, auto&& load) {
+                        load(a, &G.x, s * 64, i0);
+                        load(b, wm, s * 64, j0);
+                        if (!PAIR) load(b + HB, &G.w[1], s * 64, j0);
+                    });
+                } else if (w.mode == FF_DX) {
+                    run([&](int s, uint32_t a, uint32_t b, auto&& load) {
+                        const int g = s >= half, k0 = (s - g * half) * 64;
+                        load(a, &G.dguk[g], k0, i0);
+                        load(b, &G.w[g], j0, k0);
+                        load(b + HB, &G.w[g], j0 + 64, k0);
+                    });
+                } else {
+                    const CUtensorMap* am = &G.dgum[it.part];
+                    run([&](int s, uint32_t a, uint32_t b, auto&& load) {
+                        load(a, am, i0, s * 64);
+                        load(a + HB, am, i0 + 64, s * 64);
+                        load(b, &G.x, j0, s * 64);
+                        load(b + HB, &G.x, j0 + 64, s * 64);
+                    });
                 }
             }
             // no copy of either CTA is still landing (all complete on the leader's barriers)
@@ -222,64 +284,80 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
-            constexpr int AMN = MODE == FF_DW, BMN = MODE != FF_FORWARD;
-            uint32_t idesc = idesc_bf16(256, FN, AMN, BMN);
-            if (G.dtype == SCAO_F16) idesc &= ~((1u << 7) | (1u << 10));
             int stage = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
-            for (int T = cid; T < total && !abort_flag; T += ncl) {
+            for (int n = 0; !abort_flag && ff_item(G, grp, ngrp, n, it); ++n) {
+                const FfWork& w = G.work[it.w];
                 if (!mbar_wait(&acce[acc], aph ^ 1)) { abort_flag = 1; ff_fail(G.status); break; }
                 tc_fence_after();
-                const uint32_t d = tmem + acc * FN;
+                const uint32_t d = tmem + acc * TN;
+                const bool amn = !FORWARD && w.mode == FF_DW;
+                uint32_t idesc = idesc_bf16(TM, TN, 0, FORWARD ? 0 : 1) | (amn ? 1u << 15 : 0u);
+                if (G.dtype == SCAO_F16) idesc &= ~((1u << 7) | (1u << 10));
+                const int s0 = ff_first(w, it.split), s1 = ff_first(w, it.split + 1);
                 bool ok = true;
-                for (int s = 0; s < steps; ++s) {
-                    if (!mbar_wait(&full[stage], ph)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t a = smem_u32(sm + (size_t)stage * FSTAGE), b = a + FOPB;
+                auto run = [&](auto a_mn) {
+                    // 16 deep: 32 bytes along a K-major row, 2 KB of MN-major rows
+                    constexpr bool AMN = decltype(a_mn)::value;
+                    const uint64_t ad0 = AMN ? smem_desc_sw128(smem_u32(sm), FOPB / 2, 1024)
+                                             : smem_desc_sw128(smem_u32(sm), 16, 1024);
+                    const uint64_t bd0 = FORWARD ? smem_desc_sw128(smem_u32(sm) + FOPB, 16, 1024)
+                                                 : smem_desc_sw128(smem_u32(sm) + FOPB, FOPB / 2, 1024);
+                    for (int s = s0; s < s1; ++s) {
+                        if (!mbar_wait(&full[stage], ph)) { ok = false; return; }
+                        tc_fence_after();
+                        const uint64_t at = (uint64_t)stage * (FSTAGE >> 4);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        // 16 deep: 32 bytes along a K-major row, 2 KB of MN-major rows
-                        const uint64_t ad = AMN ? smem_desc_sw128(a + k * 2048, FOPB / 2, 1024)
-                                                : smem_desc_sw128(a + k * 32, 16, 1024);
-                        const uint64_t bd = BMN ? smem_desc_sw128(b + k * 2048, FOPB / 2, 1024)
-                                                : smem_desc_sw128(b + k * 32, 16, 1024);
-                        tc_mma_bf16_pair(d, ad, bd, idesc, (s > 0 || k > 0) ? 1u : 0u);
+                        for (int k = 0; k < 4; ++k) {
+                            const uint64_t ad = ad0 + at + k * (AMN ? 2048 >> 4 : 32 >> 4);
+                            const uint64_t bd = bd0 + at + k * (FORWARD ? 32 >> 4 : 2048 >> 4);
+                            const uint32_t more = (s > s0 || k > 0) ? 1u : 0u;
+                            if (PAIR) tc_mma_bf16_pair(d, ad, bd, idesc, more);
+                            else tc_mma_bf16(d, ad, bd, idesc, more);
+                        }
+                        commit(&empty[stage]);
+                        if (++stage == FST) { stage = 0; ph ^= 1; }
                     }
-                    tc_commit_pair(&empty[stage], 0x3);
-                    if (++stage == FST) { stage = 0; ph ^= 1; }
-                }
+                };
+                if (amn) run(std::true_type()); else run(std::false_type());
                 if (!ok) { abort_flag = 1; ff_fail(G.status); break; }
-                tc_commit_pair(&accf[acc], 0x3);
+                commit(&accf[acc]);
                 acc ^= 1;
                 if (acc == 0) aph ^= 1;
             }
-            tc_commit_pair(&fin, 0x3);
+            commit(&fin);
         }
         __syncwarp();
         if (!mbar_wait(&fin, 0)) ff_fail(G.status);
-    } else {
+    } else if (warp - 2 < EPI) {
         const int q = warp & 3, h = (warp - 2) >> 2;     // TMEM lane quarter, column half
         unsigned char* stage = sm + (size_t)FST * FSTAGE + (warp - 2) * FOUTB;
-        const uint32_t acce_cl[2] = {mapa_shared(smem_u32(&acce[0]), 0),
-                                     mapa_shared(smem_u32(&acce[1]), 0)};
         int acc = 0;
         uint32_t aph = 0;
-        for (int T = cid; T < total; T += ncl) {
+        auto release = [&] {                             // this warp has read the accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_cl(mapa_shared(smem_u32(&acce[acc]), 0));
+                else mbar_arrive(&acce[acc]);
+            }
+        };
+        for (int n = 0; ff_item(G, grp, ngrp, n, it); ++n) {
             if (__any_sync(0xffffffffu, abort_flag)) break;
-            const FfTile w = ff_tile(G, T);
+            const FfWork& w = G.work[it.w];
             if (!__all_sync(0xffffffffu, mbar_wait(&accf[acc], aph))) {
                 abort_flag = 1;
                 ff_fail(G.status);
                 break;
             }
             tc_fence_after();
-            const int row0 = w.m * 256 + 128 * (int)rank + q * 32, row = row0 + lane;
-            const uint32_t tb = tmem + acc * FN + ((uint32_t)(q * 32) << 16);
-            if (MODE == FF_FORWARD) {
-                const int c0 = w.n * 128 + h * 64, cb = (G.cols + 127) >> 7;
+            const int row0 = it.m * TM + 128 * (int)rank + q * 32, row = row0 + lane;
+            const uint32_t tb = tmem + acc * TN + ((uint32_t)(q * 32) << 16);
+            if constexpr (FORWARD) {
+                const int c0 = it.n * (TN / 2) + h * 64, cb = (w.cols + 127) >> 7;
                 uint32_t out[32], gr[2][16], ur[2][16];
                 tc_ld16_async(tb + h * 64, gr[0]);
-                tc_ld16_async(tb + 128 + h * 64, ur[0]);
+                tc_ld16_async(tb + TN / 2 + h * 64, ur[0]);
 #pragma unroll
                 for (int c = 0; c < 64; c += 16) {      // the next 16 columns are on their way
                     uint32_t *g = gr[(c >> 4) & 1], *u = ur[(c >> 4) & 1];
@@ -287,9 +365,9 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
                     tc_ld16_wait(u);
                     if (c + 16 < 64) {
                         tc_ld16_async(tb + h * 64 + c + 16, gr[((c >> 4) + 1) & 1]);
-                        tc_ld16_async(tb + 128 + h * 64 + c + 16, ur[((c >> 4) + 1) & 1]);
+                        tc_ld16_async(tb + TN / 2 + h * 64 + c + 16, ur[((c >> 4) + 1) & 1]);
                     }
-                    if (G.saved && row < G.rows && c0 + c < G.cols) {
+                    if (G.saved && row < w.rows && c0 + c < w.cols) {
                         float* p = G.saved + saved_off(row, c0 + c, cb);
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
@@ -304,28 +382,68 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) out[(c + i) / 2] = pack2(y[i], y[i + 1], G.dtype);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cl(acce_cl[acc]);
-                ff_store_block(G, 0, out, stage, row0, c0, lane);
+                release();
+                ff_store_block(w, &G.out[0], 0, out, stage, row0, c0, lane);
             } else {
+                constexpr int COLS = TN / 2;            // of this warp
+                const int cw = h * COLS;
+                const CUtensorMap* map = &G.out[w.mode == FF_DX ? 0 : 1 + it.part];
+                if (w.splits == 1) {
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    const int c0 = h * 128 + half * 64;
-                    uint32_t out[32];
+                    for (int c0 = 0; c0 < COLS; c0 += 64) {
+                        uint32_t out[32], v[2][16];
+                        tc_ld16_async(tb + cw + c0, v[0]);
 #pragma unroll
-                    for (int c = 0; c < 64; c += 16) {
+                        for (int c = 0; c < 64; c += 16) {
+                            uint32_t* y = v[(c >> 4) & 1];
+                            tc_ld16_wait(y);
+                            if (c + 16 < 64) tc_ld16_async(tb + cw + c0 + c + 16, v[((c >> 4) + 1) & 1]);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2)
+                                out[(c + i) / 2] = pack2(__uint_as_float(y[i]), __uint_as_float(y[i + 1]), G.dtype);
+                        }
+                        if (c0 + 64 == COLS) release();
+                        ff_store_block(w, map, it.part, out, stage, row0, it.n * TN + cw + c0, lane);
+                    }
+                } else {
+                    // a share of the sum goes to memory; the warp that brings the last one adds
+                    // them all in their order, whichever came last
+                    const int64_t slot = ((int64_t)it.tile * NC + rank) * FEPI_WARPS + (warp - 2);
+                    constexpr int64_t PART = 32 * COLS;
+                    float* mine = G.partial + w.partial0 + (slot * w.splits + it.split) * PART;
+#pragma unroll 1
+                    for (int c = 0; c < COLS; c += 16) {
                         float v[16];
-                        tc_ld16(tb + c0 + c, v);
+                        tc_ld16(tb + cw + c, v);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) out[(c + i) / 2] = pack2(v[i], v[i + 1], G.dtype);
+                        for (int i = 0; i < 16; i += 4)
+                            *(float4*)(mine + ((c + i) / 4 * 32 + lane) * 4) =
+                                make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                     }
-                    if (half == 1) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cl(acce_cl[acc]);
+                    release();
+                    __threadfence();
+                    __syncwarp();
+                    int done = 0;
+                    if (lane == 0) done = atomicAdd(G.count + w.count0 + slot, 1);
+                    if (__shfl_sync(0xffffffffu, done, 0) == w.splits - 1) {
+                        __threadfence();
+                        const float* all = mine - it.split * PART;
+#pragma unroll 1
+                        for (int c0 = 0; c0 < COLS; c0 += 64) {
+                            uint32_t out[32];
+#pragma unroll
+                            for (int c = 0; c < 64; c += 4) {
+                                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                                for (int p = 0; p < w.splits; ++p) {
+                                    const float4 z = __ldcg((const float4*)(all + p * PART) + (c0 + c) / 4 * 32 + lane);
+                                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+                                }
+                                out[c / 2] = pack2(y.x, y.y, G.dtype);
+                                out[c / 2 + 1] = pack2(y.z, y.w, G.dtype);
+                            }
+                            ff_store_block(w, map, it.part, out, stage, row0, it.n * TN + cw + c0, lane);
+                        }
                     }
-                    ff_store_block(G, w.part, out, stage, row0, w.n * FN + c0, lane);
                 }
             }
             acc ^= 1;
@@ -335,34 +453,40 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync_all();
+    sync_all();
     tc_fence_after();
-    if (warp == 1) tc_dealloc_pair(tmem, 2 * FN);
+    if (warp == 1) { if (PAIR) tc_dealloc_pair(tmem, 2 * TN); else tc_dealloc(tmem, 2 * TN); }
 }
 
-// dg = dh u act'(g), du = dh act(g).  A warp takes 4 rows x 32 columns at a time:
-// runs of 64 bytes and more of every array.  HBM bound (14 bytes a value).
+// dg = dh u act'(g), du = dh act(g).  A block takes one 128 x 128 block of g and u as
+// they were kept; a warp 8 rows x 16 columns at a time: runs of 128 bytes of g and u and
+// of 32 of the others.  HBM bound (14 bytes a value): 4096 x 8192 in PW_US us, a copy of
+// as many bytes takes 77.  (4 rows x 32 columns took 90, 2 x 64 94, 1 x 128 111 us.)
 constexpr int PT = 256;
 
 template <int ACT>
-__global__ void __launch_bounds__(PT)
+__global__ void __launch_bounds__(PT, 4)
 ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict__ dh, int64_t lddh,
                     uint16_t* __restrict__ dg, uint16_t* __restrict__ du, int64_t ldg, int rows,
-                    int cols, int dtype, int vec) {
+                    int cols, int dtype, int vec, int* count, int n_count) {
+    // the counters of the products that follow
+    for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * PT + threadIdx.x; i < n_count;
+         i += gridDim.x * gridDim.y * PT)
+        count[i] = 0;
     const int cb = (cols + 127) >> 7, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c = blockIdx.y * 128 + (warp & 3) * 32 + (lane & 7) * 4;
+    const int c = blockIdx.y * 128 + warp * 16 + (lane & 3) * 4;
     if (c >= cols) return;
-    const int r0 = blockIdx.x * 128 + (warp >> 2) * 64 + (lane >> 3);
+    const int r0 = blockIdx.x * 128 + (lane >> 2);
 #pragma unroll 1
-    for (int i = 0; i < 16; i += 4) {
-        if (r0 + 4 * i >= rows) break;
-        float4 g[4], u[4], y[4];
+    for (int i = 0; i < 128; i += 16) {
+        if (r0 + i >= rows) break;
+        float4 g[2], u[2], y[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {                   // all loads first
-            const int r = min(r0 + 4 * (i + k), rows - 1);
+        for (int k = 0; k < 2; ++k) {                   // all loads first
+            const int r = min(r0 + i + 8 * k, rows - 1);
             const float* p = saved + saved_off(r, c, cb);
-            g[k] = ldg_stream4(p);
-            u[k] = ldg_stream4(p + SAVED_U);
+            g[k] = *(const float4*)p;
+            u[k] = *(const float4*)(p + SAVED_U);
             const uint16_t* d = dh + r * lddh + c;
             if (vec) {
                 y[k] = load4_dt(d, 0, dtype);
@@ -374,8 +498,8 @@ ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict_
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int r = r0 + 4 * (i + k);
+        for (int k = 0; k < 2; ++k) {
+            const int r = r0 + i + 8 * k;
             if (r >= rows) break;
             float4 a, b;
             ff_act_grad<ACT>(g[k].x, a.x, b.x);
@@ -492,24 +616,105 @@ ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-bool map2d(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int dtype, int bx,
-           int by) {
-    return scao_tensor_map_2d(m, dtype, base, rows, cols, ld, bx, by);
-}
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+int up(int64_t n, int k) { return (int)((n + k - 1) / k); }
 
-template <int MODE, int ACT = 0>
-int launch_gemm(FfGemm& G, cudaStream_t st) {
+template <bool PAIR, bool FORWARD, int ACT>
+int launch_gemm(const FfGemm& G, int items, cudaStream_t st) {
     static PerDeviceOnce once;
-    if (once.first() && cudaFuncSetAttribute(ff_gemm_kernel<MODE, ACT>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FSMEM) != cudaSuccess)
+    auto* kernel = ff_gemm_kernel<PAIR, FORWARD, ACT>;
+    if (once.first() && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)FSMEM) != cudaSuccess)
         return SCAO_ERR_LAUNCH;
-    const int64_t tiles = (int64_t)G.parts * G.mt * G.nt;
-    if (tiles > (1 << 30)) return SCAO_ERR_ARG;
-    const int pairs = scao_sm_count() / 2;
+    const int groups = scao_sm_count() / (PAIR ? 2 : 1);
     ProfScope p(SLOT_GATED_FF, st);
-    ff_gemm_kernel<MODE, ACT><<<2 * (int)(tiles < pairs ? tiles : pairs), FTHREADS, FSMEM, st>>>(G);
+    kernel<<<(items < groups ? items : groups) * (PAIR ? 2 : 1), FTHREADS, FSMEM, st>>>(G);
     SCAO_CHECK_LAUNCH();
     return SCAO_OK;
+}
+
+// How a call's products are cut.  128 x 128 tiles of single CTAs where all of them run
+// at once: they spread few rows or columns over more SMs (33 x 2048 x 8192 forward: TIME_S us,
+// against TIME_P for 256 x 256 pairs), else pairs, which read half the operand bytes for a
+// result.  Of the gradient's products, what then leaves SMs idle is split along the
+// contraction into items of at least 4 steps.
+struct FfPlan {
+    bool pair;
+    FfWork dx, dw;
+    int dx_items, dw_items;
+    int64_t partial_floats, counts;
+};
+
+int64_t tiles_of(int64_t parts, int64_t rows, int64_t cols, int t) {
+    return parts * ((rows + t - 1) / t) * ((cols + t - 1) / t);
+}
+
+FfPlan plan_backward(int rows, int d, int ff, bool want_dx, bool want_dw) {
+    FfPlan p;
+    memset(&p, 0, sizeof(p));
+    const int sms = scao_sm_count();
+    const int64_t singles = (want_dx ? tiles_of(1, rows, d, 128) : 0) + (want_dw ? tiles_of(2, ff, d, 128) : 0);
+    p.pair = singles > sms;
+    const int t = p.pair ? 256 : 128, groups = p.pair ? sms / 2 : sms;
+    auto set = [&](FfWork& w, int mode, int parts, int r, int steps) {
+        w.mode = mode;
+        w.parts = parts;
+        w.mt = up(r, t);
+        w.nt = up(d, t);
+        w.splits = 1;
+        w.steps = steps;
+        w.rows = r;
+        w.cols = d;
+        w.ldo = d;
+        return parts * w.mt * w.nt;
+    };
+    const int nx = want_dx ? set(p.dx, FF_DX, 1, rows, 2 * up(ff, 64)) : 0;
+    const int nw = want_dw ? set(p.dw, FF_DW, 2, ff, up(rows, 64)) : 0;
+    if (nx + nw < groups) {
+        // the shortest items (in steps) whose number still fits
+        const int64_t all = (int64_t)nx * p.dx.steps + (int64_t)nw * p.dw.steps;
+        const int most = nx && p.dx.steps > p.dw.steps ? p.dx.steps : p.dw.steps;
+        for (int64_t len = all / groups > 4 ? all / groups : 4; len < most; ++len) {
+            const int sx = nx ? up(p.dx.steps, (int)len) : 1, sw = nw ? up(p.dw.steps, (int)len) : 1;
+            if ((int64_t)nx * sx + (int64_t)nw * sw > groups) continue;
+            if (nx) p.dx.splits = sx;
+            if (nw) p.dw.splits = sw;
+            break;
+        }
+    }
+    const int64_t per_tile = (int64_t)t * t, warps = (p.pair ? 2 : 1) * FEPI_WARPS;
+    if (p.dx.splits > 1) {
+        p.partial_floats = nx * p.dx.splits * per_tile;
+        p.counts = nx * warps;
+    }
+    p.dw.partial0 = p.partial_floats;
+    p.dw.count0 = (int)p.counts;
+    if (p.dw.splits > 1) {
+        p.partial_floats += nw * p.dw.splits * per_tile;
+        p.counts += nw * warps;
+    }
+    p.dx_items = nx * p.dx.splits;
+    p.dw_items = nw * p.dw.splits;
+    return p;
+}
+
+// workspace: dg, du, the counters, the partial sums
+struct FfSpace { int64_t du, count, partial, bytes; };
+
+FfSpace space_of(const FfPlan& p, int rows, int ff) {
+    FfSpace s;
+    s.du = (int64_t)rows * up8(ff) * 2;
+    s.count = 2 * s.du;
+    s.partial = (s.count + p.counts * 4 + 15) / 16 * 16;
+    s.bytes = s.partial + p.partial_floats * 4;
+    return s;
+}
+
+bool map_operand(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, int dtype, int box) {
+    return scao_tensor_map_2d(m, dtype, base, rows, cols, ld, 64, box);
+}
+bool map_result(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int dtype) {
+    return scao_tensor_map_2d(m, dtype, base, rows, cols, cols, 64, 32);
 }
 
 // Host word that the kernels write when a wait runs out and that the next call
@@ -567,9 +772,6 @@ bool operands_ok(const ScaoGatedFf* f) {
            f->ldx >= (f->rows ? f->d : 0) && f->ldg >= f->d && f->ldu >= f->d;
 }
 
-int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
-int up(int64_t n, int k) { return (int)((n + k - 1) / k); }
-
 }  // namespace
 
 extern "C" int* scao_gated_ff_status_word(void) { return status_word(); }
@@ -579,8 +781,12 @@ extern "C" int64_t scao_gated_ff_saved_bytes(int rows, int ff) {
 }
 
 extern "C" int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff) {
-    (void)d;
-    return 2 * (int64_t)rows * up8(ff) * 2 + 16;
+    int64_t most = 0;
+    for (int k = 1; k < 4; ++k) {
+        const int64_t n = space_of(plan_backward(rows, d, ff, k & 1, k & 2), rows, ff).bytes;
+        if (n > most) most = n;
+    }
+    return most;
 }
 
 extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
@@ -588,94 +794,107 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     if (f->rows == 0) return SCAO_OK;
     if (!f->h) return SCAO_ERR_ARG;
     if (int rc = take_status()) return rc;
+    const cudaStream_t st = (cudaStream_t)stream;
     if (!f->saved && f->rows <= SK_ROWS) {
-        const cudaStream_t st = (cudaStream_t)stream;
         if (f->act == SCAO_ACT_SILU) return launch_skinny<SCAO_ACT_SILU>(f, st);
         if (f->act == SCAO_ACT_GELU) return launch_skinny<SCAO_ACT_GELU>(f, st);
         return launch_skinny<SCAO_ACT_GELU_TANH>(f, st);
     }
     FfGemm G;
     memset(&G, 0, sizeof(G));
-    G.tma_out = aligned(f->h, f->ff);
-    if (!map2d(&G.a[0], f->x, f->rows, f->d, f->ldx, f->dtype, 64, 128) ||
-        !map2d(&G.b[0], f->w_gate, f->ff, f->d, f->ldg, f->dtype, 64, 128) ||
-        !map2d(&G.b[1], f->w_up, f->ff, f->d, f->ldu, f->dtype, 64, 128) ||
-        (G.tma_out && !map2d(&G.out[0], f->h, f->rows, f->ff, f->ff, f->dtype, 64, 32)))
+    const bool pair = tiles_of(1, f->rows, 2 * (int64_t)f->ff, 128) > scao_sm_count();
+    FfWork& w = G.work[0];
+    w.mode = FF_FORWARD;
+    w.mt = up(f->rows, pair ? 256 : 128);
+    w.nt = up(f->ff, pair ? 128 : 64);
+    w.parts = w.splits = G.work[1].splits = 1;
+    w.steps = up(f->d, 64);
+    w.rows = f->rows;
+    w.cols = f->ff;
+    w.ldo = f->ff;
+    w.outp[0] = f->h;
+    w.tma_out = aligned(f->h, f->ff);
+    const int64_t items = (int64_t)w.mt * w.nt;
+    if (items > 1 << 30) return SCAO_ERR_ARG;
+    if (!map_operand(&G.x, f->x, f->rows, f->d, f->ldx, f->dtype, 128) ||
+        !map_operand(&G.w[0], f->w_gate, f->ff, f->d, f->ldg, f->dtype, pair ? 128 : 64) ||
+        !map_operand(&G.w[1], f->w_up, f->ff, f->d, f->ldu, f->dtype, pair ? 128 : 64) ||
+        (w.tma_out && !map_result(&G.out[0], f->h, f->rows, f->ff, f->dtype)))
         return SCAO_ERR_LAUNCH;
-    G.outp[0] = f->h;
     G.saved = (float*)f->saved;
     G.status = status_word();
-    G.ldo = f->ff;
-    G.rows = f->rows;
-    G.cols = f->ff;
-    G.mt = up(f->rows, 256);
-    G.nt = up(f->ff, 128);
-    G.parts = G.segs = 1;
-    G.ksteps = up(f->d, 64);
     G.dtype = f->dtype;
-    const cudaStream_t st = (cudaStream_t)stream;
-    if (f->act == SCAO_ACT_SILU) return launch_gemm<FF_FORWARD, SCAO_ACT_SILU>(G, st);
-    if (f->act == SCAO_ACT_GELU) return launch_gemm<FF_FORWARD, SCAO_ACT_GELU>(G, st);
-    return launch_gemm<FF_FORWARD, SCAO_ACT_GELU_TANH>(G, st);
+    const int n = (int)items;
+    if (f->act == SCAO_ACT_SILU)
+        return pair ? launch_gemm<true, true, SCAO_ACT_SILU>(G, n, st) : launch_gemm<false, true, SCAO_ACT_SILU>(G, n, st);
+    if (f->act == SCAO_ACT_GELU)
+        return pair ? launch_gemm<true, true, SCAO_ACT_GELU>(G, n, st) : launch_gemm<false, true, SCAO_ACT_GELU>(G, n, st);
+    return pair ? launch_gemm<true, true, SCAO_ACT_GELU_TANH>(G, n, st)
+                : launch_gemm<false, true, SCAO_ACT_GELU_TANH>(G, n, st);
 }
 
 extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
     if (!operands_ok(f) || f->rows == 0 || !f->saved || !f->dh || f->lddh < 0 || !f->workspace ||
-        ((uintptr_t)f->workspace & 15) || (!f->dw_gate != !f->dw_up))
+        ((uintptr_t)f->workspace & 15) || (!f->dw_gate != !f->dw_up) || up(f->ff, 128) > 65535)
         return SCAO_ERR_ARG;
     if (int rc = take_status()) return rc;
     const cudaStream_t st = (cudaStream_t)stream;
+    const bool want_dx = f->dx != nullptr, want_dw = f->dw_gate != nullptr;
+    if (!want_dx && !want_dw) return SCAO_OK;
+    FfPlan p = plan_backward(f->rows, f->d, f->ff, want_dx, want_dw);
+    if ((int64_t)p.dx.mt * p.dx.nt > 1 << 28 || 2 * (int64_t)p.dw.mt * p.dw.nt > 1 << 28) return SCAO_ERR_ARG;
+    const FfSpace space = space_of(p, f->rows, f->ff);
     const int64_t ld = up8(f->ff);
-    uint16_t *dg = (uint16_t*)f->workspace, *du = dg + f->rows * ld;
+    char* ws = (char*)f->workspace;
+    uint16_t *dg = (uint16_t*)ws, *du = (uint16_t*)(ws + space.du);
     {
         const int vec = ((uintptr_t)f->dh & 7) == 0 && (f->lddh & 3) == 0 && (f->ff & 3) == 0;
-        if (up(f->ff, 128) > 65535) return SCAO_ERR_ARG;
-        ProfScope p(SLOT_GATED_FF, st);
+        ProfScope prof(SLOT_GATED_FF, st);
         auto* kernel = f->act == SCAO_ACT_SILU   ? ff_pointwise_kernel<SCAO_ACT_SILU>
                        : f->act == SCAO_ACT_GELU ? ff_pointwise_kernel<SCAO_ACT_GELU>
                                                  : ff_pointwise_kernel<SCAO_ACT_GELU_TANH>;
         kernel<<<dim3(up(f->rows, 128), up(f->ff, 128)), PT, 0, st>>>(
-            (const float*)f->saved, (const uint16_t*)f->dh, f->lddh, dg, du, ld, f->rows, f->ff, f->dtype, vec);
+            (const float*)f->saved, (const uint16_t*)f->dh, f->lddh, dg, du, ld, f->rows, f->ff, f->dtype, vec,
+            (int*)(ws + space.count), (int)p.counts);
         SCAO_CHECK_LAUNCH();
     }
     FfGemm G;
     memset(&G, 0, sizeof(G));
     G.status = status_word();
     G.dtype = f->dtype;
-    G.ldo = G.cols = f->d;
-    G.nt = up(f->d, FN);
-    if (f->dx) {
-        G.tma_out = aligned(f->dx, f->d);
-        if (!map2d(&G.a[0], dg, f->rows, f->ff, ld, f->dtype, 64, 128) ||
-            !map2d(&G.a[1], du, f->rows, f->ff, ld, f->dtype, 64, 128) ||
-            !map2d(&G.b[0], f->w_gate, f->ff, f->d, f->ldg, f->dtype, 64, 64) ||
-            !map2d(&G.b[1], f->w_up, f->ff, f->d, f->ldu, f->dtype, 64, 64) ||
-            (G.tma_out && !map2d(&G.out[0], f->dx, f->rows, f->d, f->d, f->dtype, 64, 32)))
+    G.count = (int*)(ws + space.count);
+    G.partial = (float*)(ws + space.partial);
+    if (want_dx) {
+        if (!map_operand(&G.w[0], f->w_gate, f->ff, f->d, f->ldg, f->dtype, 64) ||
+            !map_operand(&G.w[1], f->w_up, f->ff, f->d, f->ldu, f->dtype, 64) ||
+            !map_operand(&G.dguk[0], dg, f->rows, f->ff, ld, f->dtype, 128) ||
+            !map_operand(&G.dguk[1], du, f->rows, f->ff, ld, f->dtype, 128))
             return SCAO_ERR_LAUNCH;
-        G.outp[0] = f->dx;
-        G.rows = f->rows;
-        G.mt = up(f->rows, 256);
-        G.parts = 1;
-        G.segs = 2;
-        G.ksteps = up(f->ff, 64);
-        if (int rc = launch_gemm<FF_DX>(G, st)) return rc;
+        p.dx.outp[0] = f->dx;
+        p.dx.tma_out = aligned(f->dx, f->d);
+        if (p.dx.tma_out && !map_result(&G.out[0], f->dx, f->rows, f->d, f->dtype)) return SCAO_ERR_LAUNCH;
     }
-    if (f->dw_gate) {
-        G.tma_out = aligned(f->dw_gate, f->d) && aligned(f->dw_up, f->d);
-        if (!map2d(&G.a[0], dg, f->rows, f->ff, ld, f->dtype, 64, 64) ||
-            !map2d(&G.a[1], du, f->rows, f->ff, ld, f->dtype, 64, 64) ||
-            !map2d(&G.b[0], f->x, f->rows, f->d, f->ldx, f->dtype, 64, 64) ||
-            (G.tma_out && (!map2d(&G.out[0], f->dw_gate, f->ff, f->d, f->d, f->dtype, 64, 32) ||
-                           !map2d(&G.out[1], f->dw_up, f->ff, f->d, f->d, f->dtype, 64, 32))))
+    if (want_dw) {
+        if (!map_operand(&G.x, f->x, f->rows, f->d, f->ldx, f->dtype, 64) ||
+            !map_operand(&G.dgum[0], dg, f->rows, f->ff, ld, f->dtype, 64) ||
+            !map_operand(&G.dgum[1], du, f->rows, f->ff, ld, f->dtype, 64))
             return SCAO_ERR_LAUNCH;
-        G.outp[0] = f->dw_gate;
-        G.outp[1] = f->dw_up;
-        G.rows = f->ff;
-        G.mt = up(f->ff, 256);
-        G.parts = 2;
-        G.segs = 1;
-        G.ksteps = up(f->rows, 64);
-        if (int rc = launch_gemm<FF_DW>(G, st)) return rc;
+        p.dw.outp[0] = f->dw_gate;
+        p.dw.outp[1] = f->dw_up;
+        p.dw.tma_out = aligned(f->dw_gate, f->d) && aligned(f->dw_up, f->d);
+        if (p.dw.tma_out && (!map_result(&G.out[1], f->dw_gate, f->ff, f->d, f->dtype) ||
+                             !map_result(&G.out[2], f->dw_up, f->ff, f->d, f->dtype)))
+            return SCAO_ERR_LAUNCH;
     }
-    return SCAO_OK;
+    // the product with the longer items first
+    const int lx = want_dx ? p.dx.steps / p.dx.splits : 0, lw = want_dw ? p.dw.steps / p.dw.splits : 0;
+    const bool dx_first = lx >= lw;
+    G.work[0] = dx_first ? p.dx : p.dw;
+    G.work[1] = dx_first ? p.dw : p.dx;
+    for (FfWork& w : G.work)
+        if (!w.splits) w.splits = 1;                    // not wanted: no tiles
+    const int a = dx_first ? lx : lw, b = dx_first ? lw : lx;
+    G.extra = b ? (a + b / 2) / b : 0;
+    const int items = p.dx_items + p.dw_items;
+    return p.pair ? launch_gemm<true, false, 0>(G, items, st) : launch_gemm<false, false, 0>(G, items, st);
 }

@@ -125,9 +125,12 @@ def test_every_small_row_count(m):
     check(*inputs(m, 136, 72, torch.float16), "silu", False)
 
 
-def test_many_tiles():
-    """More tiles than SM pairs: the persistent loop and both accumulators."""
-    check(*inputs(2100, 320, 1500, torch.bfloat16), "silu", True)
+@pytest.mark.parametrize("m,d,f", [(2100, 320, 1500), (1500, 700, 1600), (3000, 1100, 2100), (600, 2000, 700),
+                                   (5000, 136, 136), (200, 64, 9000), (9000, 64, 200)])
+def test_many_tiles(m, d, f):
+    """More tiles than SMs: the persistent loop and both accumulators; results of one CTA
+    and of pairs, whole and split contractions, either product the longer one."""
+    check(*inputs(m, d, f, torch.bfloat16), "silu", True)
 
 
 def test_long_contraction():
