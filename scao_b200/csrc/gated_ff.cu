@@ -34,15 +34,26 @@ namespace {
 
 enum { FF_FORWARD = 0, FF_DX, FF_DW };      // what a work item computes
 
-constexpr int FST = 6;                      // pipeline stages
-constexpr uint32_t FOPB = 128 * 64 * 2;     // one 128 x 64 operand block, 16 KB: two TMA boxes of 64 x 64
-constexpr uint32_t FSTAGE = 2 * FOPB;
+// Tiles: of one CTA, or of the two CTAs of a cluster (tcgen05.mma.cta_group::2), of which
+// each stages its 128 (TALL: 256) rows of A and 128 columns of B.
+enum { SINGLE = 0 /* 128 x 128 */, PAIR /* 256 x 256 */, TALL /* 512 x 256 */ };
+
+constexpr uint32_t FOPB = 128 * 64 * 2;     // one 128 x 64 operand block, 16 KB
 constexpr int FEPI_WARPS = 8;
 constexpr uint32_t FOUTB = 32 * 64 * 2;     // a warp's 32 x 64 block of the result, 4 KB
 constexpr int FTHREADS = 64 + 32 * FEPI_WARPS;
-constexpr int FBAND = 16;                   // row tiles per band of the tile order
-constexpr size_t FSMEM = 1024 + (size_t)FST * FSTAGE + FEPI_WARPS * FOUTB;
-static_assert(FSMEM <= 231 * 1024, "shared memory");
+constexpr int FBAND_ROWS = 4096;            // rows per band of the tile order
+
+template <int SHAPE>
+struct FfShape {
+    static constexpr int NC = SHAPE == SINGLE ? 1 : 2;      // CTAs of a tile
+    static constexpr int HALVES = SHAPE == TALL ? 2 : 1;    // 128-row blocks of A in a CTA
+    static constexpr int TM = 128 * NC * HALVES, TN = 128 * NC;
+    static constexpr uint32_t STAGE = (HALVES + 1) * FOPB;
+    static constexpr int STAGES = SHAPE == TALL ? 4 : 6;    // 192 KB either way
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + FEPI_WARPS * FOUTB;
+};
+static_assert(FfShape<TALL>::SMEM <= 231 * 1024 && FfShape<PAIR>::SMEM <= 231 * 1024, "shared memory");
 
 // One product: `parts` results of rows x cols in mt x nt tiles, each the sum over
 // `steps` 64-deep blocks, which `splits` items share.
@@ -72,6 +83,7 @@ struct FfItem { int w, part, m, n, split, tile; };
 // The n-th item of group g of G (a CTA or a pair): items of work[0] in turn, then those
 // of work[1].  Where the first do not come out even, the groups that got one less
 // take `extra` items of the second first: about as many as take the same time.
+template <int BAND>
 SCAO_DEV bool ff_item(const FfGemm& P, int g, int G, int n, FfItem& it) {
     const FfWork &a = P.work[0], &b = P.work[1];
     const int na = a.parts * a.mt * a.nt * a.splits, nb = b.parts * b.mt * b.nt * b.splits;
@@ -100,13 +112,13 @@ found:
     const int per = w.mt * w.nt;
     it.part = it.tile / per;
     int t = it.tile - it.part * per;
-    // in bands of FBAND row tiles, row tiles fastest: the tiles that run at one time
-    // share few operand panels, which stay in L2
-    const int band = t / (FBAND * w.nt);
-    t -= band * FBAND * w.nt;
-    const int h = min(FBAND, w.mt - band * FBAND);
+    // in bands of row tiles, row tiles fastest: the tiles that run at one time share few
+    // operand panels, which stay in L2
+    const int band = t / (BAND * w.nt);
+    t -= band * BAND * w.nt;
+    const int h = min(BAND, w.mt - band * BAND);
     it.n = t / h;
-    it.m = band * FBAND + t - it.n * h;
+    it.m = band * BAND + t - it.n * h;
     return true;
 }
 
@@ -189,29 +201,36 @@ SCAO_DEV void ff_store_block(const FfWork& w, const CUtensorMap* map, int part, 
     __syncwarp();
 }
 
-// One tcgen05 product kernel: a CTA (128 x 128 tiles) or, PAIR, the two CTAs of a
-// cluster (256 x 256 tiles, tcgen05.mma.cta_group::2, each CTA staging 128 rows of A
-// and 128 of B).  Roles per CTA: warp 0 TMA producer; warp 1 TMEM owner and (first CTA)
-// MMA issuer; warps 2-9 epilogue, which overlaps the next item's main loop (two
-// accumulators).  Every wait is bounded; when one runs out the CTA records it in
-// *status, issues no more, waits for its copies in flight, and both CTAs still meet at
-// the end.
-template <bool PAIR, bool FORWARD, int ACT>
-__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(FTHREADS, 1)
+// The product kernel.  Roles per CTA: warp 0 TMA producer; warp 1 TMEM owner and (first
+// CTA) MMA issuer; warps 2-9 epilogue, which overlaps the next item's main loop.  TMEM
+// holds two accumulators of 128 rows x TN columns per CTA: of alternate items, or, TALL,
+// of the two row halves of one item.  TALL reads a quarter less for a result; its
+// halves share every stage, so around the end of an item the order of the MMAs changes:
+// a pipeline's length of the first half's last steps, then the second half's, then the
+// same of the next item, which gives the epilogue that long for each half
+// while the tensor cores go on.
+// Every wait is bounded; when one runs out the CTA records it in *status, issues no
+// more, waits for its copies in flight, and both CTAs still meet at the end.
+template <int SHAPE, bool FORWARD, int ACT>
+__global__ void __cluster_dims__(SHAPE == SINGLE ? 1 : 2, 1, 1) __launch_bounds__(FTHREADS, 1)
 ff_gemm_kernel(const __grid_constant__ FfGemm G) {
-    constexpr int NC = PAIR ? 2 : 1, TM = 128 * NC, TN = 128 * NC;
+    typedef FfShape<SHAPE> Sh;
+    constexpr bool TWO = Sh::NC == 2;
+    constexpr int NC = Sh::NC, HALVES = Sh::HALVES, TM = Sh::TM, TN = Sh::TN, FST = Sh::STAGES;
+    constexpr uint32_t FSTAGE = Sh::STAGE;
+    constexpr int BAND = FBAND_ROWS / TM;
     // the forward tile of one CTA has 64 columns: four warps read it
-    constexpr int EPI = FORWARD && !PAIR ? 4 : FEPI_WARPS;
+    constexpr int EPI = FORWARD && !TWO ? 4 : FEPI_WARPS;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = (unsigned char*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[FST], empty[FST], accf[2], acce[2], fin;
     __shared__ uint32_t tslot;
     __shared__ volatile int abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+    const uint32_t rank = TWO ? cluster_ctarank() : 0;
     const bool leader = rank == 0;
-    auto sync_all = [] { if (PAIR) cluster_sync_all(); else __syncthreads(); };
-    auto commit = [](uint64_t* bar) { if (PAIR) tc_commit_pair(bar, 0x3); else tc_commit(bar); };
+    auto sync_all = [] { if (TWO) cluster_sync_all(); else __syncthreads(); };
+    auto commit = [](uint64_t* bar) { if (TWO) tc_commit_pair(bar, 0x3); else tc_commit(bar); };
     if (tid == 0) {
         for (int i = 0; i < FST; ++i) { mbar_init(&full[i], NC); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&accf[i], 1); mbar_init(&acce[i], NC * EPI); }
@@ -219,7 +238,7 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) { if (PAIR) tc_alloc_pair(&tslot, 2 * TN); else tc_alloc(&tslot, 2 * TN); }
+    if (warp == 1) { if (TWO) tc_alloc_pair(&tslot, 2 * TN); else tc_alloc(&tslot, 2 * TN); }
     tc_fence_before();
     sync_all();
     tc_fence_after();
@@ -230,20 +249,20 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
         if (lane == 0) {
             int stage = 0;
             uint32_t ph = 0, issued = 0, last_ph = 0;
-            for (int n = 0; !abort_flag && ff_item(G, grp, ngrp, n, it); ++n) {
+            for (int n = 0; !abort_flag && ff_item<BAND>(G, grp, ngrp, n, it); ++n) {
                 const FfWork& w = G.work[it.w];
-                const int i0 = it.m * TM + 128 * (int)rank;
+                const int i0 = it.m * TM + 128 * (int)rank;     // of the first half; the second 256 on
                 const int j0 = FORWARD ? it.n * (TN / 2) : it.n * TN + 128 * (int)rank;
-                const int s0 = ff_first(w, it.split), s1 = ff_first(w, it.split + 1), half = w.steps >> 1;
+                const int s0 = ff_first(w, it.split), s1 = ff_first(w, it.split + 1), seg = w.steps >> 1;
                 // one step: waits for its stage, announces its bytes and lets `fill` copy them
                 auto run = [&](auto&& fill) {
                     for (int s = s0; s < s1; ++s) {
                         if (!mbar_wait(&empty[stage], ph ^ 1)) { abort_flag = 1; ff_fail(G.status); return; }
-                        const uint32_t bar = PAIR ? mapa_shared(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
-                        if (PAIR) mbar_arrive_expect_tx_cl(bar, FSTAGE); else mbar_expect_tx(&full[stage], FSTAGE);
+                        const uint32_t bar = TWO ? mapa_shared(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
+                        if (TWO) mbar_arrive_expect_tx_cl(bar, FSTAGE); else mbar_expect_tx(&full[stage], FSTAGE);
                         const uint32_t a = smem_u32(sm) + stage * FSTAGE;
-                        fill(s, a, a + FOPB, [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
-                            if (PAIR) tma_load_2d_pair(dst, map, x, y, bar);
+                        fill(s, a, a + HALVES * FOPB, [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+                            if (TWO) tma_load_2d_pair(dst, map, x, y, bar);
                             else tma_load_2d(dst, map, x, y, &full[stage]);
                         });
                         issued |= 1u << stage;
@@ -255,22 +274,27 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
                 if (FORWARD) {
                     const CUtensorMap* wm = &G.w[rank];
                     run([&](int s, uint32_t a, uint32_t b, auto&& load) {
-                        load(a, &G.x, s * 64, i0);
+#pragma unroll
+                        for (int h = 0; h < HALVES; ++h) load(a + h * FOPB, &G.x, s * 64, i0 + 256 * h);
                         load(b, wm, s * 64, j0);
-                        if (!PAIR) load(b + HB, &G.w[1], s * 64, j0);
+                        if (!TWO) load(b + HB, &G.w[1], s * 64, j0);
                     });
                 } else if (w.mode == FF_DX) {
                     run([&](int s, uint32_t a, uint32_t b, auto&& load) {
-                        const int g = s >= half, k0 = (s - g * half) * 64;
-                        load(a, &G.dguk[g], k0, i0);
+                        const int g = s >= seg, k0 = (s - g * seg) * 64;
+#pragma unroll
+                        for (int h = 0; h < HALVES; ++h) load(a + h * FOPB, &G.dguk[g], k0, i0 + 256 * h);
                         load(b, &G.w[g], j0, k0);
                         load(b + HB, &G.w[g], j0 + 64, k0);
                     });
                 } else {
                     const CUtensorMap* am = &G.dgum[it.part];
                     run([&](int s, uint32_t a, uint32_t b, auto&& load) {
-                        load(a, am, i0, s * 64);
-                        load(a + HB, am, i0 + 64, s * 64);
+#pragma unroll
+                        for (int h = 0; h < HALVES; ++h) {
+                            load(a + h * FOPB, am, i0 + 256 * h, s * 64);
+                            load(a + h * FOPB + HB, am, i0 + 256 * h + 64, s * 64);
+                        }
                         load(b, &G.x, j0, s * 64);
                         load(b + HB, &G.x, j0 + 64, s * 64);
                     });
@@ -284,47 +308,82 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
-            int stage = 0, acc = 0;
+            int stage = 0;
             uint32_t ph = 0, aph = 0;
-            for (int n = 0; !abort_flag && ff_item(G, grp, ngrp, n, it); ++n) {
-                const FfWork& w = G.work[it.w];
-                if (!mbar_wait(&acce[acc], aph ^ 1)) { abort_flag = 1; ff_fail(G.status); break; }
+            bool ok = true;
+            auto need = [&](uint64_t* bar, uint32_t parity) {
+                if (ok && !mbar_wait(bar, parity)) ok = false;
                 tc_fence_after();
-                const uint32_t d = tmem + acc * TN;
+            };
+            for (int n = 0; ok && !abort_flag && ff_item<BAND>(G, grp, ngrp, n, it); ++n) {
+                const FfWork& w = G.work[it.w];
                 const bool amn = !FORWARD && w.mode == FF_DW;
-                uint32_t idesc = idesc_bf16(TM, TN, 0, FORWARD ? 0 : 1) | (amn ? 1u << 15 : 0u);
+                uint32_t idesc = idesc_bf16(128 * NC, TN, 0, FORWARD ? 0 : 1) | (amn ? 1u << 15 : 0u);
                 if (G.dtype == SCAO_F16) idesc &= ~((1u << 7) | (1u << 10));
-                const int s0 = ff_first(w, it.split), s1 = ff_first(w, it.split + 1);
-                bool ok = true;
+                const int steps = ff_first(w, it.split + 1) - ff_first(w, it.split);
                 auto run = [&](auto a_mn) {
                     // 16 deep: 32 bytes along a K-major row, 2 KB of MN-major rows
                     constexpr bool AMN = decltype(a_mn)::value;
-                    const uint64_t ad0 = AMN ? smem_desc_sw128(smem_u32(sm), FOPB / 2, 1024)
-                                             : smem_desc_sw128(smem_u32(sm), 16, 1024);
-                    const uint64_t bd0 = FORWARD ? smem_desc_sw128(smem_u32(sm) + FOPB, 16, 1024)
-                                                 : smem_desc_sw128(smem_u32(sm) + FOPB, FOPB / 2, 1024);
-                    for (int s = s0; s < s1; ++s) {
-                        if (!mbar_wait(&full[stage], ph)) { ok = false; return; }
-                        tc_fence_after();
-                        const uint64_t at = (uint64_t)stage * (FSTAGE >> 4);
+                    const uint32_t a0 = smem_u32(sm), b0 = a0 + HALVES * FOPB;
+                    const uint64_t ad0 = AMN ? smem_desc_sw128(a0, FOPB / 2, 1024) : smem_desc_sw128(a0, 16, 1024);
+                    const uint64_t bd0 = FORWARD ? smem_desc_sw128(b0, 16, 1024) : smem_desc_sw128(b0, FOPB / 2, 1024);
+                    // the products of stage `st` into accumulator `acc`, with A's row block h
+                    auto mma = [&](int st, int h, int acc, bool first) {
+                        const uint64_t at = (uint64_t)st * (FSTAGE >> 4);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const uint64_t ad = ad0 + at + k * (AMN ? 2048 >> 4 : 32 >> 4);
+                            const uint64_t ad = ad0 + at + h * (FOPB >> 4) + k * (AMN ? 2048 >> 4 : 32 >> 4);
                             const uint64_t bd = bd0 + at + k * (FORWARD ? 32 >> 4 : 2048 >> 4);
-                            const uint32_t more = (s > s0 || k > 0) ? 1u : 0u;
-                            if (PAIR) tc_mma_bf16_pair(d, ad, bd, idesc, more);
-                            else tc_mma_bf16(d, ad, bd, idesc, more);
+                            const uint32_t more = (!first || k > 0) ? 1u : 0u;
+                            if (TWO) tc_mma_bf16_pair(tmem + acc * TN, ad, bd, idesc, more);
+                            else tc_mma_bf16(tmem + acc * TN, ad, bd, idesc, more);
                         }
-                        commit(&empty[stage]);
-                        if (++stage == FST) { stage = 0; ph ^= 1; }
+                    };
+                    if constexpr (HALVES == 1) {
+                        const int acc = n & 1;
+                        need(&acce[acc], aph ^ 1);
+                        for (int s = 0; s < steps; ++s) {
+                            need(&full[stage], ph);
+                            if (!ok) return;
+                            mma(stage, 0, acc, s == 0);
+                            commit(&empty[stage]);
+                            if (++stage == FST) { stage = 0; ph ^= 1; }
+                        }
+                        commit(&accf[acc]);
+                        if (acc == 1) aph ^= 1;
+                    } else {
+                        // `count` steps of the first half, then the same of the second
+                        auto block = [&](int count, bool begins, bool ends) {
+                            int st = stage;
+                            uint32_t p = ph;
+                            if (begins) need(&acce[0], aph ^ 1);
+                            for (int i = 0; i < count; ++i) {
+                                need(&full[st], p);
+                                if (!ok) return;
+                                mma(st, 0, 0, begins && i == 0);
+                                if (++st == FST) { st = 0; p ^= 1; }
+                            }
+                            if (ends) commit(&accf[0]);
+                            if (begins) need(&acce[1], aph ^ 1);
+                            if (!ok) return;
+                            for (int i = 0; i < count; ++i) {
+                                mma(stage, 1, 1, begins && i == 0);
+                                commit(&empty[stage]);
+                                if (++stage == FST) stage = 0;
+                            }
+                            ph = p;
+                            if (ends) commit(&accf[1]);
+                        };
+                        const int head = min(steps, FST), tail = min(steps - head, FST);
+                        block(head, true, tail == 0);
+                        for (int s = head; ok && s < steps - tail; ++s) block(1, false, false);
+                        if (ok && tail) block(tail, false, true);
+                        aph ^= 1;
                     }
                 };
                 if (amn) run(std::true_type()); else run(std::false_type());
-                if (!ok) { abort_flag = 1; ff_fail(G.status); break; }
-                commit(&accf[acc]);
-                acc ^= 1;
-                if (acc == 0) aph ^= 1;
             }
+            if (!ok) { abort_flag = 1; ff_fail(G.status); }
             commit(&fin);
         }
         __syncwarp();
@@ -332,41 +391,45 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
     } else if (warp - 2 < EPI) {
         const int q = warp & 3, h = (warp - 2) >> 2;     // TMEM lane quarter, column half
         unsigned char* stage = sm + (size_t)FST * FSTAGE + (warp - 2) * FOUTB;
-        int acc = 0;
         uint32_t aph = 0;
-        auto release = [&] {                             // this warp has read the accumulator
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (PAIR) mbar_arrive_cl(mapa_shared(smem_u32(&acce[acc]), 0));
-                else mbar_arrive(&acce[acc]);
-            }
-        };
-        for (int n = 0; ff_item(G, grp, ngrp, n, it); ++n) {
-            if (__any_sync(0xffffffffu, abort_flag)) break;
+        // accumulator `acc` -> the rows of A's block `half` of item `it`; false to give up
+        auto finish = [&](int acc, int half) {
             const FfWork& w = G.work[it.w];
+            if (__any_sync(0xffffffffu, abort_flag)) return false;
             if (!__all_sync(0xffffffffu, mbar_wait(&accf[acc], aph))) {
                 abort_flag = 1;
                 ff_fail(G.status);
-                break;
+                return false;
             }
             tc_fence_after();
-            const int row0 = it.m * TM + 128 * (int)rank + q * 32, row = row0 + lane;
+            auto release = [&] {                         // this warp has read the accumulator
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (TWO) mbar_arrive_cl(mapa_shared(smem_u32(&acce[acc]), 0));
+                    else mbar_arrive(&acce[acc]);
+                }
+            };
+            const int row0 = it.m * TM + 256 * half + 128 * (int)rank + q * 32, row = row0 + lane;
             const uint32_t tb = tmem + acc * TN + ((uint32_t)(q * 32) << 16);
             if constexpr (FORWARD) {
                 const int c0 = it.n * (TN / 2) + h * 64, cb = (w.cols + 127) >> 7;
-                uint32_t out[32], gr[2][16], ur[2][16];
-                tc_ld16_async(tb + h * 64, gr[0]);
-                tc_ld16_async(tb + TN / 2 + h * 64, ur[0]);
+                // everything out of TMEM first, so the next item's products wait for no store
+                uint32_t gr[64], ur[64], out[32];
 #pragma unroll
-                for (int c = 0; c < 64; c += 16) {      // the next 16 columns are on their way
-                    uint32_t *g = gr[(c >> 4) & 1], *u = ur[(c >> 4) & 1];
-                    tc_ld16_wait(g);
-                    tc_ld16_wait(u);
-                    if (c + 16 < 64) {
-                        tc_ld16_async(tb + h * 64 + c + 16, gr[((c >> 4) + 1) & 1]);
-                        tc_ld16_async(tb + TN / 2 + h * 64 + c + 16, ur[((c >> 4) + 1) & 1]);
-                    }
+                for (int c = 0; c < 64; c += 16) {
+                    tc_ld16_async(tb + h * 64 + c, gr + c);
+                    tc_ld16_async(tb + TN / 2 + h * 64 + c, ur + c);
+                }
+#pragma unroll
+                for (int c = 0; c < 64; c += 16) {
+                    tc_ld16_wait(gr + c);
+                    tc_ld16_wait(ur + c);
+                }
+                release();
+#pragma unroll
+                for (int c = 0; c < 64; c += 16) {
+                    const uint32_t *g = gr + c, *u = ur + c;
                     if (G.saved && row < w.rows && c0 + c < w.cols) {
                         float* p = G.saved + saved_off(row, c0 + c, cb);
 #pragma unroll
@@ -382,33 +445,31 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) out[(c + i) / 2] = pack2(y[i], y[i + 1], G.dtype);
                 }
-                release();
                 ff_store_block(w, &G.out[0], 0, out, stage, row0, c0, lane);
             } else {
                 constexpr int COLS = TN / 2;            // of this warp
                 const int cw = h * COLS;
                 const CUtensorMap* map = &G.out[w.mode == FF_DX ? 0 : 1 + it.part];
                 if (w.splits == 1) {
-#pragma unroll 1
-                    for (int c0 = 0; c0 < COLS; c0 += 64) {
-                        uint32_t out[32], v[2][16];
-                        tc_ld16_async(tb + cw + c0, v[0]);
+                    uint32_t out[COLS / 2], v[2][16];
+                    tc_ld16_async(tb + cw, v[0]);
 #pragma unroll
-                        for (int c = 0; c < 64; c += 16) {
-                            uint32_t* y = v[(c >> 4) & 1];
-                            tc_ld16_wait(y);
-                            if (c + 16 < 64) tc_ld16_async(tb + cw + c0 + c + 16, v[((c >> 4) + 1) & 1]);
+                    for (int c = 0; c < COLS; c += 16) {        // the next 16 columns are on their way
+                        uint32_t* y = v[(c >> 4) & 1];
+                        tc_ld16_wait(y);
+                        if (c + 16 < COLS) tc_ld16_async(tb + cw + c + 16, v[((c >> 4) + 1) & 1]);
 #pragma unroll
-                            for (int i = 0; i < 16; i += 2)
-                                out[(c + i) / 2] = pack2(__uint_as_float(y[i]), __uint_as_float(y[i + 1]), G.dtype);
-                        }
-                        if (c0 + 64 == COLS) release();
-                        ff_store_block(w, map, it.part, out, stage, row0, it.n * TN + cw + c0, lane);
+                        for (int i = 0; i < 16; i += 2)
+                            out[(c + i) / 2] = pack2(__uint_as_float(y[i]), __uint_as_float(y[i + 1]), G.dtype);
                     }
+                    release();
+#pragma unroll
+                    for (int c0 = 0; c0 < COLS; c0 += 64)
+                        ff_store_block(w, map, it.part, out + c0 / 2, stage, row0, it.n * TN + cw + c0, lane);
                 } else {
                     // a share of the sum goes to memory; the warp that brings the last one adds
                     // them all in their order, whichever came last
-                    const int64_t slot = ((int64_t)it.tile * NC + rank) * FEPI_WARPS + (warp - 2);
+                    const int64_t slot = (((int64_t)it.tile * NC + rank) * HALVES + half) * FEPI_WARPS + (warp - 2);
                     constexpr int64_t PART = 32 * COLS;
                     float* mine = G.partial + w.partial0 + (slot * w.splits + it.split) * PART;
 #pragma unroll 1
@@ -446,8 +507,19 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
                     }
                 }
             }
-            acc ^= 1;
-            if (acc == 0) aph ^= 1;
+            return true;
+        };
+        for (int n = 0; ff_item<BAND>(G, grp, ngrp, n, it); ++n) {
+            if constexpr (HALVES == 1) {
+                if (!finish(n & 1, 0)) break;
+                if (n & 1) aph ^= 1;
+            } else {
+                bool more = true;
+#pragma unroll 1
+                for (int half = 0; more && half < 2; ++half) more = finish(half, half);
+                if (!more) break;
+                aph ^= 1;
+            }
         }
         if (lane == 0) bulk_wait0();        // the stores have left shared memory and are visible
     }
@@ -455,7 +527,7 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
     __syncthreads();
     sync_all();
     tc_fence_after();
-    if (warp == 1) { if (PAIR) tc_dealloc_pair(tmem, 2 * TN); else tc_dealloc(tmem, 2 * TN); }
+    if (warp == 1) { if (TWO) tc_dealloc_pair(tmem, 2 * TN); else tc_dealloc(tmem, 2 * TN); }
 }
 
 // dg = dh u act'(g), du = dh act(g).  A block takes one 128 x 128 block of g and u as
@@ -619,70 +691,88 @@ ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 int up(int64_t n, int k) { return (int)((n + k - 1) / k); }
 
-template <bool PAIR, bool FORWARD, int ACT>
-int launch_gemm(const FfGemm& G, int items, cudaStream_t st) {
+template <int SHAPE, bool FORWARD, int ACT>
+int launch_shape(const FfGemm& G, int items, cudaStream_t st) {
     static PerDeviceOnce once;
-    auto* kernel = ff_gemm_kernel<PAIR, FORWARD, ACT>;
-    if (once.first() && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)FSMEM) != cudaSuccess)
+    auto* kernel = ff_gemm_kernel<SHAPE, FORWARD, ACT>;
+    constexpr int NC = FfShape<SHAPE>::NC, SMEM = (int)FfShape<SHAPE>::SMEM;
+    if (once.first() && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
         return SCAO_ERR_LAUNCH;
-    const int groups = scao_sm_count() / (PAIR ? 2 : 1);
+    const int groups = scao_sm_count() / NC;
     ProfScope p(SLOT_GATED_FF, st);
-    kernel<<<(items < groups ? items : groups) * (PAIR ? 2 : 1), FTHREADS, FSMEM, st>>>(G);
+    kernel<<<(items < groups ? items : groups) * NC, FTHREADS, SMEM, st>>>(G);
     SCAO_CHECK_LAUNCH();
     return SCAO_OK;
 }
 
-// How a call's products are cut.  128 x 128 tiles of single CTAs where all of them run
-// at once: they spread few rows or columns over more SMs (33 x 2048 x 8192 forward: TIME_S us,
-// against TIME_P for 256 x 256 pairs), else pairs, which read half the operand bytes for a
-// result.  Of the gradient's products, what then leaves SMs idle is split along the
-// contraction into items of at least 4 steps.
-struct FfPlan {
-    bool pair;
-    FfWork dx, dw;
-    int dx_items, dw_items;
-    int64_t partial_floats, counts;
-};
-
-int64_t tiles_of(int64_t parts, int64_t rows, int64_t cols, int t) {
-    return parts * ((rows + t - 1) / t) * ((cols + t - 1) / t);
+template <bool FORWARD, int ACT>
+int launch_gemm(int shape, const FfGemm& G, int items, cudaStream_t st) {
+    if (shape == SINGLE) return launch_shape<SINGLE, FORWARD, ACT>(G, items, st);
+    if (shape == PAIR) return launch_shape<PAIR, FORWARD, ACT>(G, items, st);
+    return launch_shape<TALL, FORWARD, ACT>(G, items, st);
 }
 
-FfPlan plan_backward(int rows, int d, int ff, bool want_dx, bool want_dw) {
+int tile_rows(int shape) { return shape == SINGLE ? 128 : shape == PAIR ? 256 : 512; }
+int tile_cols(int shape) { return shape == SINGLE ? 128 : 256; }
+int group_count(int shape) { return scao_sm_count() / (shape == SINGLE ? 1 : 2); }
+
+// Steps that the busiest group runs, as ff_item deals the items out: na of la steps, then
+// nb of lb.
+int64_t longest(int64_t na, int64_t la, int64_t nb, int64_t lb, int extra, int G) {
+    const int64_t h = na / G, r = na % G, early = r ? (G - r) * extra < nb ? (G - r) * extra : nb : 0;
+    const int64_t rest = (nb - early + G - 1) / G * lb;
+    const int64_t x = (h + (r > 0)) * la + rest, y = h * la + (early ? extra : 0) * lb + rest;
+    return x > y ? x : y;
+}
+
+// Time of a step of a tile, relative: TALL 1024 clocks of the tensor cores, PAIR 512, of
+// which the operands' way from L2 makes about STEP_P; see plan_shape.
+double step_cost(int shape) { return shape == TALL ? 1.0 : 0.65; }
+
+struct FfPlan {
+    int shape;
+    FfWork dx, dw;
+    int dx_items, dw_items, extra;
+    bool dx_first;
+    int64_t partial_floats, counts;
+    double cost;
+};
+
+// The gradient's products in tiles of one shape.  Where the tiles are fewer than the
+// groups, they are split along the contraction into items of at least 4 steps.
+FfPlan plan_shape(int shape, int rows, int d, int ff, bool want_dx, bool want_dw) {
     FfPlan p;
     memset(&p, 0, sizeof(p));
-    const int sms = scao_sm_count();
-    const int64_t singles = (want_dx ? tiles_of(1, rows, d, 128) : 0) + (want_dw ? tiles_of(2, ff, d, 128) : 0);
-    p.pair = singles > sms;
-    const int t = p.pair ? 256 : 128, groups = p.pair ? sms / 2 : sms;
+    p.shape = shape;
+    const int tm = tile_rows(shape), tn = tile_cols(shape), groups = group_count(shape);
     auto set = [&](FfWork& w, int mode, int parts, int r, int steps) {
         w.mode = mode;
         w.parts = parts;
-        w.mt = up(r, t);
-        w.nt = up(d, t);
+        w.mt = up(r, tm);
+        w.nt = up(d, tn);
         w.splits = 1;
         w.steps = steps;
         w.rows = r;
         w.cols = d;
         w.ldo = d;
-        return parts * w.mt * w.nt;
+        return (int64_t)parts * w.mt * w.nt;
     };
-    const int nx = want_dx ? set(p.dx, FF_DX, 1, rows, 2 * up(ff, 64)) : 0;
-    const int nw = want_dw ? set(p.dw, FF_DW, 2, ff, up(rows, 64)) : 0;
+    p.dx.splits = p.dw.splits = 1;
+    const int64_t nx = want_dx ? set(p.dx, FF_DX, 1, rows, 2 * up(ff, 64)) : 0;
+    const int64_t nw = want_dw ? set(p.dw, FF_DW, 2, ff, up(rows, 64)) : 0;
     if (nx + nw < groups) {
         // the shortest items (in steps) whose number still fits
-        const int64_t all = (int64_t)nx * p.dx.steps + (int64_t)nw * p.dw.steps;
-        const int most = nx && p.dx.steps > p.dw.steps ? p.dx.steps : p.dw.steps;
+        const int64_t all = nx * p.dx.steps + nw * p.dw.steps;
+        const int most = p.dx.steps > p.dw.steps ? p.dx.steps : p.dw.steps;
         for (int64_t len = all / groups > 4 ? all / groups : 4; len < most; ++len) {
             const int sx = nx ? up(p.dx.steps, (int)len) : 1, sw = nw ? up(p.dw.steps, (int)len) : 1;
-            if ((int64_t)nx * sx + (int64_t)nw * sw > groups) continue;
-            if (nx) p.dx.splits = sx;
-            if (nw) p.dw.splits = sw;
+            if (nx * sx + nw * sw > groups) continue;
+            p.dx.splits = sx;
+            p.dw.splits = sw;
             break;
         }
     }
-    const int64_t per_tile = (int64_t)t * t, warps = (p.pair ? 2 : 1) * FEPI_WARPS;
+    const int64_t per_tile = (int64_t)tm * tn, warps = tm / 128 * FEPI_WARPS;
     if (p.dx.splits > 1) {
         p.partial_floats = nx * p.dx.splits * per_tile;
         p.counts = nx * warps;
@@ -693,9 +783,42 @@ FfPlan plan_backward(int rows, int d, int ff, bool want_dx, bool want_dw) {
         p.partial_floats += nw * p.dw.splits * per_tile;
         p.counts += nw * warps;
     }
-    p.dx_items = nx * p.dx.splits;
-    p.dw_items = nw * p.dw.splits;
+    const int64_t ix = nx * p.dx.splits, iw = nw * p.dw.splits;
+    if (ix + iw > 1 << 30) p.cost = -1;                  // refused
+    p.dx_items = (int)ix;
+    p.dw_items = (int)iw;
+    // the product with the longer items first
+    const int lx = nx ? up(p.dx.steps, p.dx.splits) : 0, lw = nw ? up(p.dw.steps, p.dw.splits) : 0;
+    p.dx_first = lx >= lw;
+    const int a = p.dx_first ? lx : lw, b = p.dx_first ? lw : lx;
+    p.extra = b ? (a + b / 2) / b : 0;
+    if (p.cost == 0)
+        p.cost = step_cost(shape) * (double)(p.dx_first ? longest(ix, a, iw, b, p.extra, groups)
+                                                        : longest(iw, a, ix, b, p.extra, groups));
     return p;
+}
+
+int64_t tiles_of(int64_t parts, int64_t rows, int64_t cols, int tm, int tn) {
+    return parts * ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn);
+}
+
+// Tiles of single CTAs where all of them run at once: they spread few rows or columns over
+// more SMs.  Else the pairs' shape whose busiest pair is done first.
+FfPlan plan_backward(int rows, int d, int ff, bool want_dx, bool want_dw) {
+    if ((want_dx ? tiles_of(1, rows, d, 128, 128) : 0) + (want_dw ? tiles_of(2, ff, d, 128, 128) : 0) <=
+        scao_sm_count())
+        return plan_shape(SINGLE, rows, d, ff, want_dx, want_dw);
+    const FfPlan p = plan_shape(PAIR, rows, d, ff, want_dx, want_dw), t = plan_shape(TALL, rows, d, ff, want_dx, want_dw);
+    return t.cost <= p.cost ? t : p;
+}
+
+int plan_forward(int rows, int ff) {
+    const int64_t one = tiles_of(1, rows, ff, 128, 64);
+    if (one <= scao_sm_count()) return SINGLE;
+    const int64_t p = tiles_of(1, rows, ff, 256, 128), t = tiles_of(1, rows, ff, 512, 128);
+    const int groups = group_count(PAIR);
+    return step_cost(TALL) * (double)((t + groups - 1) / groups) <= step_cost(PAIR) * (double)((p + groups - 1) / groups)
+               ? TALL : PAIR;
 }
 
 // workspace: dg, du, the counters, the partial sums
@@ -802,11 +925,11 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     }
     FfGemm G;
     memset(&G, 0, sizeof(G));
-    const bool pair = tiles_of(1, f->rows, 2 * (int64_t)f->ff, 128) > scao_sm_count();
+    const int shape = plan_forward(f->rows, f->ff), box = shape == SINGLE ? 64 : 128;
     FfWork& w = G.work[0];
     w.mode = FF_FORWARD;
-    w.mt = up(f->rows, pair ? 256 : 128);
-    w.nt = up(f->ff, pair ? 128 : 64);
+    w.mt = up(f->rows, tile_rows(shape));
+    w.nt = up(f->ff, tile_cols(shape) / 2);
     w.parts = w.splits = G.work[1].splits = 1;
     w.steps = up(f->d, 64);
     w.rows = f->rows;
@@ -817,20 +940,17 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     const int64_t items = (int64_t)w.mt * w.nt;
     if (items > 1 << 30) return SCAO_ERR_ARG;
     if (!map_operand(&G.x, f->x, f->rows, f->d, f->ldx, f->dtype, 128) ||
-        !map_operand(&G.w[0], f->w_gate, f->ff, f->d, f->ldg, f->dtype, pair ? 128 : 64) ||
-        !map_operand(&G.w[1], f->w_up, f->ff, f->d, f->ldu, f->dtype, pair ? 128 : 64) ||
+        !map_operand(&G.w[0], f->w_gate, f->ff, f->d, f->ldg, f->dtype, box) ||
+        !map_operand(&G.w[1], f->w_up, f->ff, f->d, f->ldu, f->dtype, box) ||
         (w.tma_out && !map_result(&G.out[0], f->h, f->rows, f->ff, f->dtype)))
         return SCAO_ERR_LAUNCH;
     G.saved = (float*)f->saved;
     G.status = status_word();
     G.dtype = f->dtype;
     const int n = (int)items;
-    if (f->act == SCAO_ACT_SILU)
-        return pair ? launch_gemm<true, true, SCAO_ACT_SILU>(G, n, st) : launch_gemm<false, true, SCAO_ACT_SILU>(G, n, st);
-    if (f->act == SCAO_ACT_GELU)
-        return pair ? launch_gemm<true, true, SCAO_ACT_GELU>(G, n, st) : launch_gemm<false, true, SCAO_ACT_GELU>(G, n, st);
-    return pair ? launch_gemm<true, true, SCAO_ACT_GELU_TANH>(G, n, st)
-                : launch_gemm<false, true, SCAO_ACT_GELU_TANH>(G, n, st);
+    if (f->act == SCAO_ACT_SILU) return launch_gemm<true, SCAO_ACT_SILU>(shape, G, n, st);
+    if (f->act == SCAO_ACT_GELU) return launch_gemm<true, SCAO_ACT_GELU>(shape, G, n, st);
+    return launch_gemm<true, SCAO_ACT_GELU_TANH>(shape, G, n, st);
 }
 
 extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
@@ -842,7 +962,7 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
     const bool want_dx = f->dx != nullptr, want_dw = f->dw_gate != nullptr;
     if (!want_dx && !want_dw) return SCAO_OK;
     FfPlan p = plan_backward(f->rows, f->d, f->ff, want_dx, want_dw);
-    if ((int64_t)p.dx.mt * p.dx.nt > 1 << 28 || 2 * (int64_t)p.dw.mt * p.dw.nt > 1 << 28) return SCAO_ERR_ARG;
+    if (p.cost < 0) return SCAO_ERR_ARG;
     const FfSpace space = space_of(p, f->rows, f->ff);
     const int64_t ld = up8(f->ff);
     char* ws = (char*)f->workspace;
@@ -886,15 +1006,8 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
                              !map_result(&G.out[2], f->dw_up, f->ff, f->d, f->dtype)))
             return SCAO_ERR_LAUNCH;
     }
-    // the product with the longer items first
-    const int lx = want_dx ? p.dx.steps / p.dx.splits : 0, lw = want_dw ? p.dw.steps / p.dw.splits : 0;
-    const bool dx_first = lx >= lw;
-    G.work[0] = dx_first ? p.dx : p.dw;
-    G.work[1] = dx_first ? p.dw : p.dx;
-    for (FfWork& w : G.work)
-        if (!w.splits) w.splits = 1;                    // not wanted: no tiles
-    const int a = dx_first ? lx : lw, b = dx_first ? lw : lx;
-    G.extra = b ? (a + b / 2) / b : 0;
-    const int items = p.dx_items + p.dw_items;
-    return p.pair ? launch_gemm<true, false, 0>(G, items, st) : launch_gemm<false, false, 0>(G, items, st);
+    G.work[0] = p.dx_first ? p.dx : p.dw;
+    G.work[1] = p.dx_first ? p.dw : p.dx;
+    G.extra = p.extra;
+    return launch_gemm<false, 0>(p.shape, G, p.dx_items + p.dw_items, st);
 }

@@ -126,7 +126,8 @@ def test_every_small_row_count(m):
 
 
 @pytest.mark.parametrize("m,d,f", [(2100, 320, 1500), (1500, 700, 1600), (3000, 1100, 2100), (600, 2000, 700),
-                                   (5000, 136, 136), (200, 64, 9000), (9000, 64, 200)])
+                                   (5000, 136, 136), (200, 64, 9000), (9000, 64, 200),
+                                   (4000, 72, 4000), (4100, 700, 2500)])
 def test_many_tiles(m, d, f):
     """More tiles than SMs: the persistent loop and both accumulators; results of one CTA
     and of pairs, whole and split contractions, either product the longer one."""
