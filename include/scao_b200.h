@@ -460,7 +460,11 @@ SCAO_API int scao_rotary(const ScaoRotary* args, void* stream);
  * `saved` (scao_gated_ff_saved_bytes; null if no gradient will be taken)
  * keeps what backward reads.  backward: from dh (row pitch lddh) to dx and to
  * dw_gate and dw_up (null: not wanted, the two together), with a workspace
- * of scao_gated_ff_workspace_bytes, 16-byte aligned.  A kernel whose wait
+ * of scao_gated_ff_workspace_bytes (which: 1 dx, 2 dw, 3 both), 16-byte
+ * aligned.  pack: copies up to three matrices, rows {source, copy, rows,
+ * columns, source row pitch} of the host table, to the next row pitch that
+ * is a multiple of 8 values, zeros behind each row; copies start on 16
+ * bytes.  A kernel whose wait
  * ran out sets the status word (host memory; null where there is no GPU);
  * the next call clears it and returns SCAO_ERR_TIMEOUT without launching.  */
 #define SCAO_ACT_SILU 0
@@ -475,7 +479,8 @@ typedef struct {
     int32_t rows, d, ff, dtype, act, pad0;
 } ScaoGatedFf;
 SCAO_API int64_t scao_gated_ff_saved_bytes(int rows, int ff);
-SCAO_API int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff);
+SCAO_API int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff, int which);
+SCAO_API int scao_gated_ff_pack(const int64_t* table, int n, void* stream);
 SCAO_API int* scao_gated_ff_status_word(void);
 SCAO_API int scao_gated_ff_forward(const ScaoGatedFf* args, void* stream);
 SCAO_API int scao_gated_ff_backward(const ScaoGatedFf* args, void* stream);

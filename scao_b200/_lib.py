@@ -167,7 +167,8 @@ SIGNATURES = {
     "scao_grads_overlap": (C.c_int, [_P, C.c_int]),
     "scao_rotary": (C.c_int, [_P, _P]),
     "scao_gated_ff_saved_bytes": (C.c_int64, [C.c_int, C.c_int]),
-    "scao_gated_ff_workspace_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int]),
+    "scao_gated_ff_workspace_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "scao_gated_ff_pack": (C.c_int, [_P, C.c_int, _P]),
     "scao_gated_ff_status_word": (C.POINTER(C.c_int), []),
     "scao_gated_ff_forward": (C.c_int, [_P, _P]),
     "scao_gated_ff_backward": (C.c_int, [_P, _P]),

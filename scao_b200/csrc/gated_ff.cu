@@ -58,7 +58,8 @@ static_assert(FfShape<TALL>::SMEM <= 231 * 1024 && FfShape<PAIR>::SMEM <= 231 * 
 // One product: `parts` results of rows x cols in mt x nt tiles, each the sum over
 // `steps` 64-deep blocks, which `splits` items share.
 struct FfWork {
-    int mode, parts, mt, nt, splits, steps, rows, cols, tma_out;
+    int mode, parts, mt, nt, splits, steps, rows, cols;
+    int tma_out, vec;                       // results by TMA; else by stores of 4, 2 or (1) one or two values
     int count0;                             // split: this product's first counter,
     int64_t partial0;                       // and the first of its partial sums
     int64_t ldo;
@@ -191,12 +192,34 @@ SCAO_DEV void ff_store_block(const FfWork& w, const CUtensorMap* map, int part, 
         return;
     }
     __syncwarp();
-    for (int r = 0; r < 32 && row0 + r < w.rows; ++r) {
-        uint16_t* dst = (uint16_t*)w.outp[part] + (int64_t)(row0 + r) * w.ldo;
-#pragma unroll
-        for (int c = lane; c < 64; c += 32)
-            if (col0 + c < w.cols)
-                dst[col0 + c] = *(const uint16_t*)(stage + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2);
+    // rows that are no multiple of 16 bytes apart: the widest stores that their pitch allows
+    auto at = [&](int r, int c) { return stage + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2; };
+    uint16_t* out = (uint16_t*)w.outp[part] + col0;
+    const int rows = min(32, w.rows - row0), cols = min(64, w.cols - col0);
+    if (w.vec == 4) {
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+            const int r = 2 * i + (lane >> 4), c = (lane & 15) * 4;
+            if (r < rows && c < cols) *(uint2*)(out + (row0 + r) * w.ldo + c) = *(const uint2*)at(r, c);
+        }
+    } else if (w.vec == 2) {
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r)
+            if (r < rows && 2 * lane < cols)
+                *(uint32_t*)(out + (row0 + r) * w.ldo + 2 * lane) = *(const uint32_t*)at(r, 2 * lane);
+    } else {
+        // an odd pitch: every other row begins between two 32-bit words
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r) {
+            uint16_t* d = out + (row0 + r) * w.ldo;
+            const int odd = ((uintptr_t)d >> 1) & 1, c = 2 * lane + odd;
+            if (r >= rows) continue;
+            if (odd && lane == 0 && cols > 0) d[0] = *(const uint16_t*)at(r, 0);
+            if (c >= cols) continue;
+            const uint32_t x = *(const uint16_t*)at(r, c);
+            if (c + 1 < cols) *(uint32_t*)(d + c) = x | (uint32_t)*(const uint16_t*)at(r, c + 1) << 16;
+            else d[c] = (uint16_t)x;
+        }
     }
     __syncwarp();
 }
@@ -491,17 +514,26 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
                         const float* all = mine - it.split * PART;
 #pragma unroll 1
                         for (int c0 = 0; c0 < COLS; c0 += 64) {
+                            float y[64];
+#pragma unroll
+                            for (int i = 0; i < 64; ++i) y[i] = 0.f;
+#pragma unroll 2
+                            for (int p = 0; p < w.splits; ++p) {
+                                const float4* z = (const float4*)(all + p * PART) + c0 * 8 + lane;
+                                float4 t[16];               // one share's loads together
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) t[i] = __ldcg(z + i * 32);
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    y[4 * i] += t[i].x;
+                                    y[4 * i + 1] += t[i].y;
+                                    y[4 * i + 2] += t[i].z;
+                                    y[4 * i + 3] += t[i].w;
+                                }
+                            }
                             uint32_t out[32];
 #pragma unroll
-                            for (int c = 0; c < 64; c += 4) {
-                                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                                for (int p = 0; p < w.splits; ++p) {
-                                    const float4 z = __ldcg((const float4*)(all + p * PART) + (c0 + c) / 4 * 32 + lane);
-                                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-                                }
-                                out[c / 2] = pack2(y.x, y.y, G.dtype);
-                                out[c / 2 + 1] = pack2(y.z, y.w, G.dtype);
-                            }
+                            for (int i = 0; i < 32; ++i) out[i] = pack2(y[2 * i], y[2 * i + 1], G.dtype);
                             ff_store_block(w, map, it.part, out, stage, row0, it.n * TN + cw + c0, lane);
                         }
                     }
@@ -530,8 +562,8 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
     if (warp == 1) { if (TWO) tc_dealloc_pair(tmem, 2 * TN); else tc_dealloc(tmem, 2 * TN); }
 }
 
-// dg = dh u act'(g), du = dh act(g).  A block takes one 128 x 128 block of g and u as
-// they were kept; a warp 8 rows x 16 columns at a time: runs of 128 bytes of g and u and
+// dg = dh u act'(g), du = dh act(g).  A block takes `span` rows of a 128-column block of
+// g and u as they were kept; a warp 8 rows x 16 columns at a time: runs of 128 bytes of g and u and
 // of 32 of the others.  HBM bound (14 bytes a value): 4096 x 8192 in PW_US us, a copy of
 // as many bytes takes 77.  (4 rows x 32 columns took 90, 2 x 64 94, 1 x 128 111 us.)
 constexpr int PT = 256;
@@ -540,7 +572,7 @@ template <int ACT>
 __global__ void __launch_bounds__(PT, 4)
 ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict__ dh, int64_t lddh,
                     uint16_t* __restrict__ dg, uint16_t* __restrict__ du, int64_t ldg, int rows,
-                    int cols, int dtype, int vec, int* count, int n_count) {
+                    int cols, int dtype, int vec, int span, int* count, int n_count) {
     // the counters of the products that follow
     for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * PT + threadIdx.x; i < n_count;
          i += gridDim.x * gridDim.y * PT)
@@ -548,9 +580,9 @@ ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict_
     const int cb = (cols + 127) >> 7, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.y * 128 + warp * 16 + (lane & 3) * 4;
     if (c >= cols) return;
-    const int r0 = blockIdx.x * 128 + (lane >> 2);
+    const int r0 = blockIdx.x * span + (lane >> 2);
 #pragma unroll 1
-    for (int i = 0; i < 128; i += 16) {
+    for (int i = 0; i < span; i += 16) {
         if (r0 + i >= rows) break;
         float4 g[2], u[2], y[2];
 #pragma unroll
@@ -622,30 +654,33 @@ SCAO_DEV uint4 load8_guard(const uint16_t* p, int left) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int ACT, bool BF16, int NT>
+template <int ACT, bool BF16, int NT, int FG>
 __global__ void __launch_bounds__(32 * SK_WARPS)
 ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ wg, int64_t ldg,
                  const uint16_t* __restrict__ wu, int64_t ldu, uint16_t* __restrict__ h, int rows, int d,
                  int ff) {
     constexpr int U = NT == 1 ? 4 : 2;          // 32-deep steps in flight
-    __shared__ float part[SK_WARPS][NT * 4][32];
+    __shared__ float part[SK_WARPS][FG * NT * 4][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int f = blockIdx.x * 8 + g;
-    const bool has = f < ff;
-    const uint16_t* pg = wg + (int64_t)min(f, ff - 1) * ldg;
-    const uint16_t* pu = wu + (int64_t)min(f, ff - 1) * ldu;
-    float acc[NT][4];
+    const int f0 = blockIdx.x * 8 * FG + g;
+    float acc[FG][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int j = 0; j < FG; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][n][i] = 0.f;
     for (int k0 = warp * 32 * U; k0 < d; k0 += SK_WARPS * 32 * U) {
-        uint4 a[U], b[U], v[NT][U];
+        uint4 a[FG][U], b[FG][U], v[NT][U];
 #pragma unroll
         for (int s = 0; s < U; ++s) {
             const int k = k0 + 32 * s + 8 * t;
-            a[s] = load8_guard(pg + k, d - k);
-            b[s] = load8_guard(pu + k, d - k);
+#pragma unroll
+            for (int j = 0; j < FG; ++j) {
+                const int64_t f = min(f0 + 8 * j, ff - 1);
+                a[j][s] = load8_guard(wg + f * ldg + k, d - k);
+                b[j][s] = load8_guard(wu + f * ldu + k, d - k);
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int r = n * 8 + g;
@@ -655,34 +690,93 @@ ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __
 #pragma unroll
         for (int s = 0; s < U; ++s)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mma_16816(acc[n], a[s].x, b[s].x, a[s].y, b[s].y, v[n][s].x, v[n][s].y, BF16);
-                mma_16816(acc[n], a[s].z, b[s].z, a[s].w, b[s].w, v[n][s].z, v[n][s].w, BF16);
-            }
+            for (int j = 0; j < FG; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint4 p = a[j][s], q = b[j][s], y = v[n][s];
+                    mma_16816(acc[j][n], p.x, q.x, p.y, q.y, y.x, y.y, BF16);
+                    mma_16816(acc[j][n], p.z, q.z, p.w, q.w, y.z, y.w, BF16);
+                }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int j = 0; j < FG; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part[warp][n * 4 + i][lane] = acc[n][i];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[warp][(j * NT + n) * 4 + i][lane] = acc[j][n][i];
     __syncthreads();
-    // thread (n, j): columns 2t + j of row group n, gate in place j and up in 2 + j
-    if (warp < NT) {
-        const int n = warp;
+    // a warp per (column group, row group); rows 2t + i, gate in place i and up in 2 + i
+    if (warp < FG * NT) {
+        const int j = warp / NT, n = warp - j * NT, f = f0 + 8 * j;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int i = 0; i < 2; ++i) {
             float gate = 0.f, upv = 0.f;
 #pragma unroll
             for (int w = 0; w < SK_WARPS; ++w) {
-                gate += part[w][n * 4 + j][lane];
-                upv += part[w][n * 4 + 2 + j][lane];
+                gate += part[w][warp * 4 + i][lane];
+                upv += part[w][warp * 4 + 2 + i][lane];
             }
-            const int r = n * 8 + 2 * t + j;
-            if (has && r < rows) {
+            const int r = n * 8 + 2 * t + i;
+            if (f < ff && r < rows) {
                 const float y = ff_act<ACT>(gate) * upv;
                 h[(int64_t)r * ff + f] = BF16 ? f_to_bf16_bits(y) : f_to_f16_bits(y);
             }
         }
     }
+}
+
+// Copies of operands whose rows TMA cannot read, at the next pitch that is a multiple of
+// 8 values, zeros behind each row: up to three matrices in one launch, a thread per 16
+// bytes written.  Where the two 16-byte words around a source run lie inside the
+// matrix they are loaded whole and shifted, else (its first and last few values) by
+// single values.
+struct FfPack {
+    const uint16_t* src[3];
+    uint16_t* dst[3];
+    int64_t pitch[3], vecs[3];              // of the source; 16-byte vectors of the copy
+    int rows[3], cols[3], n;
+};
+
+__global__ void __launch_bounds__(256)
+ff_pack_kernel(const __grid_constant__ FfPack P) {
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int m = 0;
+    while (m < P.n && i >= P.vecs[m]) i -= P.vecs[m++];
+    if (m == P.n) return;
+    const int cols = P.cols[m], per = (cols + 7) >> 3;
+    const int64_t row = i / per;
+    const int c = (int)(i - row * per) * 8, left = cols - c;
+    const uint16_t* p = P.src[m] + row * P.pitch[m] + c;
+    const uint16_t* end = P.src[m] + (P.rows[m] - 1) * P.pitch[m] + cols;
+    const int off = (int)((uintptr_t)p & 15);
+    const uint16_t* lo = p - off / 2;
+    uint4 y;
+    if (off == 0 && left >= 8) {
+        y = *(const uint4*)p;
+    } else if (lo >= P.src[m] && lo + 16 <= end) {
+        const uint4 a = *(const uint4*)lo, b = *(const uint4*)(lo + 8);
+        uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        if (off & 8)
+#pragma unroll
+            for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+        if (off & 4)
+#pragma unroll
+            for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+        if (off & 2)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)         // nothing behind the row
+            if (2 * k + 1 >= left) w[k] = 2 * k < left ? w[k] & 0xffff : 0;
+        y = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < left) w[k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
+        y = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    *(uint4*)(P.dst[m] + (row * per) * 8 + c) = y;
 }
 
 // ---------------------------------------------------------------------------
@@ -725,9 +819,12 @@ int64_t longest(int64_t na, int64_t la, int64_t nb, int64_t lb, int extra, int G
     return x > y ? x : y;
 }
 
-// Time of a step of a tile, relative: TALL 1024 clocks of the tensor cores, PAIR 512, of
-// which the operands' way from L2 makes about STEP_P; see plan_shape.
-double step_cost(int shape) { return shape == TALL ? 1.0 : 0.65; }
+// Microseconds of a step of a tile.  A CTA takes in about 50 bytes of operands a clock,
+// whatever the shape: the 32 KB of SINGLE and PAIR bound their steps (the tensor cores
+// need 256 and 512 clocks of them), the 48 KB of TALL take about its 1024 clocks.
+double step_us(int shape) { return shape == SINGLE ? 0.35 : shape == PAIR ? 0.40 : 0.72; }
+// and of joining a tile's shares
+double join_us(int shape, int splits) { return splits > 1 ? 1.5 + 0.3 * splits * (shape == PAIR ? 2 : 1) : 0; }
 
 struct FfPlan {
     int shape;
@@ -735,43 +832,31 @@ struct FfPlan {
     int dx_items, dw_items, extra;
     bool dx_first;
     int64_t partial_floats, counts;
-    double cost;
+    double us;                              // below 0: too many tiles
 };
 
-// The gradient's products in tiles of one shape.  Where the tiles are fewer than the
-// groups, they are split along the contraction into items of at least 4 steps.
-FfPlan plan_shape(int shape, int rows, int d, int ff, bool want_dx, bool want_dw) {
+// The gradient's products in tiles of one shape, dx and dW cut along the contraction
+// into so many items.
+FfPlan plan_shape(int shape, int rows, int d, int ff, int dx_splits, int dw_splits) {
     FfPlan p;
     memset(&p, 0, sizeof(p));
     p.shape = shape;
     const int tm = tile_rows(shape), tn = tile_cols(shape), groups = group_count(shape);
-    auto set = [&](FfWork& w, int mode, int parts, int r, int steps) {
+    auto set = [&](FfWork& w, int mode, int parts, int r, int steps, int splits) {
+        w.splits = splits > 0 ? splits : 1;
+        if (splits == 0) return (int64_t)0;             // not wanted
         w.mode = mode;
         w.parts = parts;
         w.mt = up(r, tm);
         w.nt = up(d, tn);
-        w.splits = 1;
         w.steps = steps;
         w.rows = r;
         w.cols = d;
         w.ldo = d;
         return (int64_t)parts * w.mt * w.nt;
     };
-    p.dx.splits = p.dw.splits = 1;
-    const int64_t nx = want_dx ? set(p.dx, FF_DX, 1, rows, 2 * up(ff, 64)) : 0;
-    const int64_t nw = want_dw ? set(p.dw, FF_DW, 2, ff, up(rows, 64)) : 0;
-    if (nx + nw < groups) {
-        // the shortest items (in steps) whose number still fits
-        const int64_t all = nx * p.dx.steps + nw * p.dw.steps;
-        const int most = p.dx.steps > p.dw.steps ? p.dx.steps : p.dw.steps;
-        for (int64_t len = all / groups > 4 ? all / groups : 4; len < most; ++len) {
-            const int sx = nx ? up(p.dx.steps, (int)len) : 1, sw = nw ? up(p.dw.steps, (int)len) : 1;
-            if (nx * sx + nw * sw > groups) continue;
-            p.dx.splits = sx;
-            p.dw.splits = sw;
-            break;
-        }
-    }
+    const int64_t nx = set(p.dx, FF_DX, 1, rows, 2 * up(ff, 64), dx_splits);
+    const int64_t nw = set(p.dw, FF_DW, 2, ff, up(rows, 64), dw_splits);
     const int64_t per_tile = (int64_t)tm * tn, warps = tm / 128 * FEPI_WARPS;
     if (p.dx.splits > 1) {
         p.partial_floats = nx * p.dx.splits * per_tile;
@@ -784,7 +869,10 @@ FfPlan plan_shape(int shape, int rows, int d, int ff, bool want_dx, bool want_dw
         p.counts += nw * warps;
     }
     const int64_t ix = nx * p.dx.splits, iw = nw * p.dw.splits;
-    if (ix + iw > 1 << 30) p.cost = -1;                  // refused
+    if (ix + iw > 1 << 30) {
+        p.us = -1;
+        return p;
+    }
     p.dx_items = (int)ix;
     p.dw_items = (int)iw;
     // the product with the longer items first
@@ -792,33 +880,56 @@ FfPlan plan_shape(int shape, int rows, int d, int ff, bool want_dx, bool want_dw
     p.dx_first = lx >= lw;
     const int a = p.dx_first ? lx : lw, b = p.dx_first ? lw : lx;
     p.extra = b ? (a + b / 2) / b : 0;
-    if (p.cost == 0)
-        p.cost = step_cost(shape) * (double)(p.dx_first ? longest(ix, a, iw, b, p.extra, groups)
-                                                        : longest(iw, a, ix, b, p.extra, groups));
+    const int most = p.dx.splits > p.dw.splits ? p.dx.splits : p.dw.splits;
+    p.us = join_us(shape, most) + step_us(shape) * (double)(p.dx_first ? longest(ix, a, iw, b, p.extra, groups)
+                                                                     : longest(iw, a, ix, b, p.extra, groups));
     return p;
 }
 
-int64_t tiles_of(int64_t parts, int64_t rows, int64_t cols, int tm, int tn) {
-    return parts * ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn);
+// The shape and the number of items whose busiest group is done first.  Where the tiles
+// leave groups idle, items of 8 steps and more are tried, in lengths a fifth apart.
+FfPlan plan_backward_new(int rows, int d, int ff, bool want_dx, bool want_dw) {
+    FfPlan best = plan_shape(TALL, rows, d, ff, want_dx, want_dw);
+    auto take = [&](const FfPlan& p) { if (best.us < 0 || (p.us >= 0 && p.us < best.us)) best = p; };
+    for (int shape = SINGLE; shape <= PAIR; ++shape) {
+        const FfPlan whole = plan_shape(shape, rows, d, ff, want_dx, want_dw);
+        take(whole);
+        const int64_t nx = whole.dx_items, nw = whole.dw_items, groups = group_count(shape);
+        if (whole.us < 0 || nx + nw >= groups) continue;
+        const int most = whole.dx.steps > whole.dw.steps ? whole.dx.steps : whole.dw.steps;
+        for (int64_t len = 8; len < most; len += len / 5 > 1 ? len / 5 : 1) {
+            const int sx = want_dx ? up(whole.dx.steps, (int)len) : 0, sw = want_dw ? up(whole.dw.steps, (int)len) : 0;
+            if (nx * sx + nw * sw <= groups) take(plan_shape(shape, rows, d, ff, sx, sw));
+        }
+    }
+    return best;
 }
 
-// Tiles of single CTAs where all of them run at once: they spread few rows or columns over
-// more SMs.  Else the pairs' shape whose busiest pair is done first.
-FfPlan plan_backward(int rows, int d, int ff, bool want_dx, bool want_dw) {
-    if ((want_dx ? tiles_of(1, rows, d, 128, 128) : 0) + (want_dw ? tiles_of(2, ff, d, 128, 128) : 0) <=
-        scao_sm_count())
-        return plan_shape(SINGLE, rows, d, ff, want_dx, want_dw);
-    const FfPlan p = plan_shape(PAIR, rows, d, ff, want_dx, want_dw), t = plan_shape(TALL, rows, d, ff, want_dx, want_dw);
-    return t.cost <= p.cost ? t : p;
+// The workspace query and the call that follows it ask for the same plan.
+const FfPlan& plan_backward(int rows, int d, int ff, bool want_dx, bool want_dw) {
+    static thread_local FfPlan plan;
+    static thread_local int of[5] = {-1, 0, 0, 0, 0};
+    const int now[5] = {rows, d, ff, want_dx, want_dw};
+    if (memcmp(of, now, sizeof(of))) {
+        plan = plan_backward_new(rows, d, ff, want_dx, want_dw);
+        memcpy(of, now, sizeof(of));
+    }
+    return plan;
+}
+
+int64_t tiles_of(int64_t rows, int64_t cols, int tm, int tn) {
+    return ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn);
 }
 
 int plan_forward(int rows, int ff) {
-    const int64_t one = tiles_of(1, rows, ff, 128, 64);
-    if (one <= scao_sm_count()) return SINGLE;
-    const int64_t p = tiles_of(1, rows, ff, 256, 128), t = tiles_of(1, rows, ff, 512, 128);
-    const int groups = group_count(PAIR);
-    return step_cost(TALL) * (double)((t + groups - 1) / groups) <= step_cost(PAIR) * (double)((p + groups - 1) / groups)
-               ? TALL : PAIR;
+    int best = SINGLE;
+    double least = 0;
+    for (int shape = SINGLE; shape <= TALL; ++shape) {
+        const int64_t n = tiles_of(rows, ff, tile_rows(shape), tile_cols(shape) / 2), g = group_count(shape);
+        const double us = step_us(shape) * (double)((n + g - 1) / g);
+        if (shape == SINGLE || us < least) best = shape, least = us;
+    }
+    return best;
 }
 
 // workspace: dg, du, the counters, the partial sums
@@ -869,11 +980,11 @@ int take_status() {
 
 template <int ACT, bool BF16>
 int launch_skinny(const ScaoGatedFf* f, cudaStream_t st) {
-    const int nt = (f->rows + 7) / 8;
-    auto* kernel = nt == 1 ? ff_skinny_kernel<ACT, BF16, 1>
-                   : nt == 2 ? ff_skinny_kernel<ACT, BF16, 2> : ff_skinny_kernel<ACT, BF16, 4>;
+    const int nt = (f->rows + 7) / 8, fg = nt > 2 ? 2 : 1;
+    auto* kernel = nt == 1 ? ff_skinny_kernel<ACT, BF16, 1, 1>
+                   : nt == 2 ? ff_skinny_kernel<ACT, BF16, 2, 1> : ff_skinny_kernel<ACT, BF16, 4, 2>;
     ProfScope p(SLOT_GATED_FF, st);
-    kernel<<<(f->ff + 7) / 8, 32 * SK_WARPS, 0, st>>>(
+    kernel<<<up(f->ff, 8 * fg), 32 * SK_WARPS, 0, st>>>(
         (const uint16_t*)f->x, f->ldx, (const uint16_t*)f->w_gate, f->ldg, (const uint16_t*)f->w_up, f->ldu,
         (uint16_t*)f->h, f->rows, f->d, f->ff);
     SCAO_CHECK_LAUNCH();
@@ -886,6 +997,15 @@ int launch_skinny(const ScaoGatedFf* f, cudaStream_t st) {
 }
 
 bool aligned(const void* p, int64_t ld) { return p && ((uintptr_t)p & 15) == 0 && ld > 0 && (ld & 7) == 0; }
+
+// how a product's packed results (one, or two) are stored
+void set_store(FfWork& w, void* a, void* b) {
+    w.outp[0] = a;
+    w.outp[1] = b;
+    const uintptr_t bits = (uintptr_t)a | (uintptr_t)b | (uintptr_t)(w.ldo * 2);
+    w.tma_out = (bits & 15) == 0;
+    w.vec = (bits & 7) == 0 ? 4 : (bits & 3) == 0 ? 2 : 1;
+}
 
 // x, Wg, Wu as TMA reads them
 bool operands_ok(const ScaoGatedFf* f) {
@@ -903,13 +1023,35 @@ extern "C" int64_t scao_gated_ff_saved_bytes(int rows, int ff) {
     return (int64_t)up(rows, 128) * up(ff, 128) * (2 * 128 * 128) * (int64_t)sizeof(float);
 }
 
-extern "C" int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff) {
-    int64_t most = 0;
-    for (int k = 1; k < 4; ++k) {
-        const int64_t n = space_of(plan_backward(rows, d, ff, k & 1, k & 2), rows, ff).bytes;
-        if (n > most) most = n;
+extern "C" int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff, int which) {
+    if (rows < 1 || d < 1 || ff < 1 || !(which & 3)) return 0;
+    return space_of(plan_backward(rows, d, ff, which & 1, which & 2), rows, ff).bytes;
+}
+
+extern "C" int scao_gated_ff_pack(const int64_t* table, int n, void* stream) {
+    if (!table || n < 1 || n > 3) return SCAO_ERR_ARG;
+    FfPack P;
+    memset(&P, 0, sizeof(P));
+    int64_t all = 0;
+    for (int i = 0; i < n; ++i) {
+        const int64_t *t = table + 5 * i, rows = t[2], cols = t[3];
+        if (!t[0] || !t[1] || (t[0] & 1) || (t[1] & 15) || rows < 1 || cols < 1 || rows > 0x7fffffff ||
+            cols > 1 << 24 || t[4] < 0)
+            return SCAO_ERR_ARG;
+        P.src[i] = (const uint16_t*)t[0];
+        P.dst[i] = (uint16_t*)t[1];
+        P.rows[i] = (int)rows;
+        P.cols[i] = (int)cols;
+        P.pitch[i] = t[4];
+        all += P.vecs[i] = rows * ((cols + 7) / 8);
     }
-    return most;
+    P.n = n;
+    if ((all + 255) / 256 > 0x7fffffff) return SCAO_ERR_ARG;
+    const cudaStream_t st = (cudaStream_t)stream;
+    ProfScope p(SLOT_GATED_FF, st);
+    ff_pack_kernel<<<(unsigned)((all + 255) / 256), 256, 0, st>>>(P);
+    SCAO_CHECK_LAUNCH();
+    return SCAO_OK;
 }
 
 extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
@@ -935,8 +1077,7 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     w.rows = f->rows;
     w.cols = f->ff;
     w.ldo = f->ff;
-    w.outp[0] = f->h;
-    w.tma_out = aligned(f->h, f->ff);
+    set_store(w, f->h, f->h);
     const int64_t items = (int64_t)w.mt * w.nt;
     if (items > 1 << 30) return SCAO_ERR_ARG;
     if (!map_operand(&G.x, f->x, f->rows, f->d, f->ldx, f->dtype, 128) ||
@@ -962,7 +1103,7 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
     const bool want_dx = f->dx != nullptr, want_dw = f->dw_gate != nullptr;
     if (!want_dx && !want_dw) return SCAO_OK;
     FfPlan p = plan_backward(f->rows, f->d, f->ff, want_dx, want_dw);
-    if (p.cost < 0) return SCAO_ERR_ARG;
+    if (p.us < 0) return SCAO_ERR_ARG;
     const FfSpace space = space_of(p, f->rows, f->ff);
     const int64_t ld = up8(f->ff);
     char* ws = (char*)f->workspace;
@@ -973,9 +1114,12 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
         auto* kernel = f->act == SCAO_ACT_SILU   ? ff_pointwise_kernel<SCAO_ACT_SILU>
                        : f->act == SCAO_ACT_GELU ? ff_pointwise_kernel<SCAO_ACT_GELU>
                                                  : ff_pointwise_kernel<SCAO_ACT_GELU_TANH>;
-        kernel<<<dim3(up(f->rows, 128), up(f->ff, 128)), PT, 0, st>>>(
+        // rows of a block: 128, fewer where that would leave SMs without one
+        int span = 128;
+        while (span > 16 && (int64_t)up(f->rows, span) * up(f->ff, 128) < 4 * scao_sm_count()) span >>= 1;
+        kernel<<<dim3(up(f->rows, span), up(f->ff, 128)), PT, 0, st>>>(
             (const float*)f->saved, (const uint16_t*)f->dh, f->lddh, dg, du, ld, f->rows, f->ff, f->dtype, vec,
-            (int*)(ws + space.count), (int)p.counts);
+            span, (int*)(ws + space.count), (int)p.counts);
         SCAO_CHECK_LAUNCH();
     }
     FfGemm G;
@@ -990,8 +1134,7 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
             !map_operand(&G.dguk[0], dg, f->rows, f->ff, ld, f->dtype, 128) ||
             !map_operand(&G.dguk[1], du, f->rows, f->ff, ld, f->dtype, 128))
             return SCAO_ERR_LAUNCH;
-        p.dx.outp[0] = f->dx;
-        p.dx.tma_out = aligned(f->dx, f->d);
+        set_store(p.dx, f->dx, f->dx);
         if (p.dx.tma_out && !map_result(&G.out[0], f->dx, f->rows, f->d, f->dtype)) return SCAO_ERR_LAUNCH;
     }
     if (want_dw) {
@@ -999,9 +1142,7 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
             !map_operand(&G.dgum[0], dg, f->rows, f->ff, ld, f->dtype, 64) ||
             !map_operand(&G.dgum[1], du, f->rows, f->ff, ld, f->dtype, 64))
             return SCAO_ERR_LAUNCH;
-        p.dw.outp[0] = f->dw_gate;
-        p.dw.outp[1] = f->dw_up;
-        p.dw.tma_out = aligned(f->dw_gate, f->d) && aligned(f->dw_up, f->d);
+        set_store(p.dw, f->dw_gate, f->dw_up);
         if (p.dw.tma_out && (!map_result(&G.out[1], f->dw_gate, f->ff, f->d, f->dtype) ||
                              !map_result(&G.out[2], f->dw_up, f->ff, f->d, f->dtype)))
             return SCAO_ERR_LAUNCH;

@@ -14,6 +14,7 @@ copied first.  ``GatedFeedForward`` is the block with its output projection.
 from __future__ import annotations
 
 import struct
+from array import array
 
 import torch
 import torch.nn as nn
@@ -28,38 +29,54 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 _ARGS = struct.Struct("@10P4q6i")
 
 
-def _rows(t):
-    """(``t`` (2-D) as the kernels read it: neighbouring values of a row adjacent, rows a
-    multiple of 16 bytes apart, the first on 16 bytes; its address; its row pitch)."""
-    n, p = t.shape[1], t.data_ptr()
-    if p & 15 == 0:
-        if n & 7 == 0 and t.is_contiguous():
-            return t, p, n
-        if t.stride(1) == 1 or n == 1:
-            pitch = t.stride(0) if t.shape[0] > 1 else (n + 7) & ~7
-            if pitch & 7 == 0 and pitch >= n:
-                return t, p, pitch
-    wide = torch.zeros(t.shape[0], (n + 7) & ~7, dtype=t.dtype, device=t.device)
-    wide[:, :n] = t
-    return wide, wide.data_ptr(), wide.shape[1]
+def _operands(tensors):
+    """The 2-D ``tensors`` as the kernels read them (neighbouring values of a row adjacent,
+    rows a multiple of 16 bytes apart, the first on 16 bytes; copies, in one launch,
+    where they lie otherwise): ([tensor, address, row pitch] of each, whether any was
+    copied)."""
+    out, table = [], []
+    for t in tensors:
+        n, p = t.shape[1], t.data_ptr()
+        if p & 15 == 0:
+            if n & 7 == 0 and t.is_contiguous():
+                out.append((t, p, n))
+                continue
+            if t.stride(1) == 1 or n == 1:
+                pitch = t.stride(0) if t.shape[0] > 1 else (n + 7) & ~7
+                if pitch & 7 == 0 and pitch >= n:
+                    out.append((t, p, pitch))
+                    continue
+        if t.stride(1) != 1:
+            t = t.contiguous()
+        wide = torch.empty((t.shape[0], (n + 7) & ~7), dtype=t.dtype, device=t.device)
+        table += (t.data_ptr(), wide.data_ptr(), t.shape[0], n, t.stride(0))
+        out.append((wide, wide.data_ptr(), wide.shape[1], t))
+    if table:
+        table = array("q", table)
+        _launch("scao_gated_ff_pack", tensors[0].get_device(), _lib.lib().scao_gated_ff_pack,
+                table.buffer_info()[0], len(table) // 5)
+    return out, bool(table)
 
 
 def _forward(x, w_gate, w_up, act, train):
-    """(h, what the gradient reads or None)."""
+    """(h, what the gradient reads or None, copies of operands or None)."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
     h = torch.empty((rows, ff), dtype=x.dtype, device=x.device)
-    saved = None
+    saved = copies = None
     if train:
         saved = torch.empty(L.scao_gated_ff_saved_bytes(rows, ff), dtype=torch.uint8, device=x.device)
     if rows:
-        (x, px, lx), (w_gate, pg, lg), (w_up, pu, lu) = _rows(x), _rows(w_gate), _rows(w_up)
-        args = _ARGS.pack(px, pg, pu, h.data_ptr(), saved.data_ptr() if train else 0, 0, 0, 0, 0, 0,
-                          lx, lg, lu, 0, rows, d, ff, _CODE[x.dtype], act, 0)
+        ins, copied = _operands((x, w_gate, w_up))
+        args = _ARGS.pack(ins[0][1], ins[1][1], ins[2][1], h.data_ptr(), saved.data_ptr() if train else 0,
+                          0, 0, 0, 0, 0, ins[0][2], ins[1][2], ins[2][2], 0,
+                          rows, d, ff, _CODE[x.dtype], act, 0)
         _launch("scao_gated_ff_forward", x.get_device(), L.scao_gated_ff_forward, args)
-    return h, saved
+        if copied and train:
+            copies = [i[0] for i in ins]
+    return h, saved, copies
 
 
-def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w):
+def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w, copies=None):
     """(dx, dw_gate, dw_up), None where not needed."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
     like = dict(dtype=x.dtype, device=x.device)
@@ -67,13 +84,15 @@ def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w):
     new = torch.empty if rows else torch.zeros
     dwg, dwu = (new((ff, d), **like), new((ff, d), **like)) if need_w else (None, None)
     if rows:
-        (x, px, lx), (w_gate, pg, lg), (w_up, pu, lu) = _rows(x), _rows(w_gate), _rows(w_up)
+        ins, _ = _operands(copies or (x, w_gate, w_up))
         if dh.stride(1) != 1:
             dh = dh.contiguous()
-        ws = torch.empty(L.scao_gated_ff_workspace_bytes(rows, d, ff), dtype=torch.uint8, device=x.device)
+        ws = torch.empty(L.scao_gated_ff_workspace_bytes(rows, d, ff, need_x | need_w << 1), dtype=torch.uint8,
+                         device=x.device)
         at = [0 if t is None else t.data_ptr() for t in (dx, dwg, dwu)]
-        args = _ARGS.pack(px, pg, pu, 0, saved.data_ptr(), dh.data_ptr(), *at, ws.data_ptr(),
-                          lx, lg, lu, dh.stride(0), rows, d, ff, _CODE[x.dtype], act, 0)
+        args = _ARGS.pack(ins[0][1], ins[1][1], ins[2][1], 0, saved.data_ptr(), dh.data_ptr(), *at,
+                          ws.data_ptr(), ins[0][2], ins[1][2], ins[2][2], dh.stride(0),
+                          rows, d, ff, _CODE[x.dtype], act, 0)
         _launch("scao_gated_ff_backward", x.get_device(), L.scao_gated_ff_backward, args)
     return dx, dwg, dwu
 
@@ -94,7 +113,7 @@ class _Once(torch.autograd.Function):
 class _GatedFF(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act):
-        h, saved = _forward(x, w_gate, w_up, act, True)
+        h, saved, ctx.copies = _forward(x, w_gate, w_up, act, True)
         ctx.act = act
         ctx.save_for_backward(x, w_gate, w_up, saved)
         return h
@@ -102,7 +121,7 @@ class _GatedFF(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dh):
         need, (x, w_gate, w_up, saved) = ctx.needs_input_grad, ctx.saved_tensors
-        grads = _backward(x, w_gate, w_up, saved, dh.detach(), ctx.act, need[0], need[1] or need[2])
+        grads = _backward(x, w_gate, w_up, saved, dh.detach(), ctx.act, need[0], need[1] or need[2], ctx.copies)
         if torch.is_grad_enabled():
             grads = [None if g is None else _Once.apply(g, x, w_gate, w_up, dh) for g in grads]
         return *grads, None
@@ -134,7 +153,7 @@ def gated_ff(x, w_gate, w_up, activation="silu"):
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         h = _GatedFF.apply(flat, w_gate, w_up, act)
     else:
-        h, _ = _forward(flat, w_gate, w_up, act, False)
+        h = _forward(flat, w_gate, w_up, act, False)[0]
     return h if x.dim() == 2 else h.view(*x.shape[:-1], w_gate.shape[0])
 
 

@@ -166,6 +166,32 @@ def test_leading_dimensions_and_strides():
             close(h.reshape(-1, f), want, err)
 
 
+@pytest.mark.parametrize("offset", range(8))
+@pytest.mark.parametrize("cols", [1, 7, 9, 16, 23, 40])
+def test_packed_copies(cols, offset):
+    """The copies of unaligned operands: every value, zeros behind the rows."""
+    from scao_b200.feedforward import _operands
+    flat = randn(40 * 50 + 64, seed=cols)
+    views = [flat[offset:offset + 40 * 49].view(40, 49)[:, :cols], flat[offset:offset + 3 * cols].view(3, cols),
+             flat[offset:offset + cols].view(1, cols)]
+    ins, _ = _operands(views)
+    torch.cuda.synchronize()
+    for (t, p, pitch, *_), v in zip(ins, views):
+        assert t.data_ptr() == p and p % 16 == 0 and pitch % 8 == 0 and torch.equal(t[:, :cols], v)
+        if t is not v:
+            assert (t[:, cols:] == 0).all()
+
+
+def test_odd_widths_keep_copies_for_the_gradient():
+    x, wg, wu = inputs(50, 43, 64, torch.bfloat16)
+    ins = [v.requires_grad_() for v in (x, wg, wu)]
+    h = gated_ff(*ins)
+    with torch.no_grad():
+        wg += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, ins, torch.ones_like(h))
+
+
 def test_values_beside_a_view_are_not_read():
     """NaN behind odd rows of x and of the weights reaches no result."""
     m, d, f = 20, 43, 50
@@ -271,7 +297,7 @@ def test_writes_nothing_else(m, f):
     guard = lambda n: torch.full((n + 1024,), 7.0, dtype=torch.bfloat16, device=DEV)  # noqa: E731
     bufs = {"h": guard(m * f), "dx": guard(m * d), "dw_gate": guard(f * d), "dw_up": guard(f * d)}
     saved = torch.empty(int(L.scao_gated_ff_saved_bytes(m, f)), dtype=torch.uint8, device=DEV)
-    ws = torch.empty(int(L.scao_gated_ff_workspace_bytes(m, d, f)), dtype=torch.uint8, device=DEV)
+    ws = torch.empty(int(L.scao_gated_ff_workspace_bytes(m, d, f, 3)), dtype=torch.uint8, device=DEV)
     dh = randn(m, f, seed=4)
     import ctypes
     a = _lib.GatedFfArgs()

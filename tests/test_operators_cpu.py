@@ -186,6 +186,16 @@ def test_gated_ff_c_entry_checks():
         assert call(L.scao_gated_ff_backward, **kw) == 1, kw
     assert L.scao_gated_ff_forward(None, None) == 1
     assert L.scao_gated_ff_saved_bytes(1, 1) == 128 * 128 * 8
+    assert L.scao_gated_ff_workspace_bytes(0, 1, 1, 3) == L.scao_gated_ff_workspace_bytes(1, 1, 1, 0) == 0
+    for which in (1, 2, 3):         # dg and du at least
+        assert L.scao_gated_ff_workspace_bytes(300, 65, 129, which) >= 2 * 2 * 300 * 136
+    good = [4096, 8192, 3, 5, 7]
+    for i, v in ((0, 0), (0, 4097), (1, 0), (1, 8200), (2, 0), (3, 0), (3, 1 << 25), (4, -1)):
+        t = array("q", good[:i] + [v] + good[i + 1:])
+        assert L.scao_gated_ff_pack(t.buffer_info()[0], 1, None) == 1, (i, v)
+    t = array("q", good * 4)
+    assert L.scao_gated_ff_pack(t.buffer_info()[0], 4, None) == 1
+    assert L.scao_gated_ff_pack(t.buffer_info()[0], 0, None) == 1
 
 
 # ----------------------------------------------------------------- the model
