@@ -111,11 +111,10 @@ def _refuse_nonfinite(total, norm_type):
                            "by it all the same")
 
 
-def _outputs(n, index):
-    """(the norm, the workspace) of ``n`` gradients."""
-    dev = torch.device("cuda", index)
-    return (torch.empty((), dtype=torch.float32, device=dev),
-            torch.empty(_lib.lib().scao_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev))
+def _outputs(tensors):
+    """(the norm, the workspace) of the gradients."""
+    t, size = tensors[0], _lib.lib().scao_grad_norm_workspace_bytes(len(tensors))
+    return t.new_empty((), dtype=torch.float32), t.new_empty(size, dtype=torch.uint8)
 
 
 def _finish(grads, packed):
@@ -139,8 +138,8 @@ def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False):
     if not tensors:
         return torch.tensor(0.0)
     n = len(tensors)
-    table, _kept, _, index = _table(tensors, write=False)
-    total, ws = _outputs(n, index)
+    table, kept, _, index = _table(tensors, write=False)
+    total, ws = _outputs(kept)
     _launch("scao_grad_norm", index, _lib.lib().scao_grad_norm, table.buffer_info()[0], n, kind,
             ws.data_ptr(), total.data_ptr())
     if error_if_nonfinite:
@@ -156,7 +155,7 @@ def clip_grads_with_norm_(parameters, max_norm, total_norm):
     grads = _grads(parameters)
     if not grads or max_norm == math.inf:
         return
-    table, _kept, packed, index = _table(grads, write=True)
+    table, kept, packed, index = _table(grads, write=True)
     if total_norm.numel() != 1 or total_norm.get_device() != index:
         raise ValueError("total_norm must be one number on the gradients' device")
     total = total_norm.detach().to(torch.float32)
@@ -180,9 +179,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if max_norm == math.inf:
         return get_total_norm(grads, norm_type, error_if_nonfinite)
     n, L = len(grads), _lib.lib()
-    table, _kept, packed, index = _table(grads, write=True)
+    table, kept, packed, index = _table(grads, write=True)
     at = table.buffer_info()[0]
-    total, ws = _outputs(n, index)
+    total, ws = _outputs(kept)
     if error_if_nonfinite:
         _launch("scao_grad_norm", index, L.scao_grad_norm, at, n, kind, ws.data_ptr(), total.data_ptr())
         _refuse_nonfinite(total, norm_type)

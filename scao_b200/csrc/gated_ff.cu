@@ -208,17 +208,21 @@ SCAO_DEV void ff_store_block(const FfWork& w, const CUtensorMap* map, int part, 
             if (r < rows && 2 * lane < cols)
                 *(uint32_t*)(out + (row0 + r) * w.ldo + 2 * lane) = *(const uint32_t*)at(r, 2 * lane);
     } else {
-        // an odd pitch: every other row begins between two 32-bit words
+        // an odd pitch: every other row begins between two 32-bit words, and a lane's
+        // word is then the upper half of its pair and the lower half of the next lane's
 #pragma unroll 4
         for (int r = 0; r < 32; ++r) {
             uint16_t* d = out + (row0 + r) * w.ldo;
             const int odd = ((uintptr_t)d >> 1) & 1, c = 2 * lane + odd;
+            uint32_t x = *(const uint32_t*)at(r, 2 * lane);
+            const uint32_t next = __shfl_down_sync(0xffffffffu, x, 1);
             if (r >= rows) continue;
-            if (odd && lane == 0 && cols > 0) d[0] = *(const uint16_t*)at(r, 0);
-            if (c >= cols) continue;
-            const uint32_t x = *(const uint16_t*)at(r, c);
-            if (c + 1 < cols) *(uint32_t*)(d + c) = x | (uint32_t)*(const uint16_t*)at(r, c + 1) << 16;
-            else d[c] = (uint16_t)x;
+            if (odd) {
+                if (lane == 0 && cols > 0) d[0] = (uint16_t)x;
+                x = __funnelshift_r(x, next, 16);
+            }
+            if (c + 1 < cols) *(uint32_t*)(d + c) = x;
+            else if (c < cols) d[c] = (uint16_t)x;
         }
     }
     __syncwarp();
@@ -262,9 +266,28 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) { if (TWO) tc_alloc_pair(&tslot, 2 * TN); else tc_alloc(&tslot, 2 * TN); }
+    if (tid == 96) {                        // the maps, on their way meanwhile
+        if (FORWARD) {
+            tc_prefetch_map(&G.x);
+            tc_prefetch_map(&G.w[0]);
+            tc_prefetch_map(&G.w[1]);
+        } else {
+            for (int i = 0; i < 2; ++i) {
+                if (G.work[i].mode == FF_DW) tc_prefetch_map(&G.x);
+                for (int k = 0; k < 2; ++k)
+                    if (G.work[i].mode == FF_DX) {
+                        tc_prefetch_map(&G.w[k]);
+                        tc_prefetch_map(&G.dguk[k]);
+                    } else if (G.work[i].mode == FF_DW) {
+                        tc_prefetch_map(&G.dgum[k]);
+                    }
+            }
+        }
+    }
     tc_fence_before();
     sync_all();
     tc_fence_after();
+    if (!FORWARD) tc_grid_wait();           // launched while the pointwise pass ran
     const uint32_t tmem = tslot;
     const int grp = blockIdx.x / NC, ngrp = gridDim.x / NC;
     FfItem it;
@@ -553,7 +576,7 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
                 aph ^= 1;
             }
         }
-        if (lane == 0) bulk_wait0();        // the stores have left shared memory and are visible
+        if (lane == 0) bulk_wait_read0();   // the stores have left shared memory
     }
     tc_fence_before();
     __syncthreads();
@@ -573,6 +596,7 @@ __global__ void __launch_bounds__(PT, 4)
 ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict__ dh, int64_t lddh,
                     uint16_t* __restrict__ dg, uint16_t* __restrict__ du, int64_t ldg, int rows,
                     int cols, int dtype, int vec, int span, int* count, int n_count) {
+    tc_grid_release();                      // the products may set up while this runs
     // the counters of the products that follow
     for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * PT + threadIdx.x; i < n_count;
          i += gridDim.x * gridDim.y * PT)
@@ -794,8 +818,20 @@ int launch_shape(const FfGemm& G, int items, cudaStream_t st) {
         return SCAO_ERR_LAUNCH;
     const int groups = scao_sm_count() / NC;
     ProfScope p(SLOT_GATED_FF, st);
-    kernel<<<(items < groups ? items : groups) * NC, FTHREADS, SMEM, st>>>(G);
-    SCAO_CHECK_LAUNCH();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((items < groups ? items : groups) * NC));
+    cfg.blockDim = dim3(FTHREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = FORWARD ? 0 : 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, G) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return SCAO_ERR_LAUNCH;
+    }
     return SCAO_OK;
 }
 

@@ -188,6 +188,16 @@ TC_DEV uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
     return smem_desc(saddr, lbo, sbo) | ((uint64_t)2 << 61);
 }
 
+// fetch a tensor map before its first use
+TC_DEV void tc_prefetch_map(const void* map) {
+    asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory");
+}
+
+// Programmatic dependent launch: a kernel lets the next one start its set-up, and the
+// next one waits until every kernel before it has finished and its writes are visible.
+TC_DEV void tc_grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+TC_DEV void tc_grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // named barrier over a subset of the CTA's warps
 TC_DEV void named_bar(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(nthreads) : "memory");

@@ -48,7 +48,7 @@ def _operands(tensors):
                     continue
         if t.stride(1) != 1:
             t = t.contiguous()
-        wide = torch.empty((t.shape[0], (n + 7) & ~7), dtype=t.dtype, device=t.device)
+        wide = t.new_empty((t.shape[0], (n + 7) & ~7))
         table += (t.data_ptr(), wide.data_ptr(), t.shape[0], n, t.stride(0))
         out.append((wide, wide.data_ptr(), wide.shape[1], t))
     if table:
@@ -61,10 +61,10 @@ def _operands(tensors):
 def _forward(x, w_gate, w_up, act, train):
     """(h, what the gradient reads or None, copies of operands or None)."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
-    h = torch.empty((rows, ff), dtype=x.dtype, device=x.device)
+    h = x.new_empty((rows, ff))
     saved = copies = None
     if train:
-        saved = torch.empty(L.scao_gated_ff_saved_bytes(rows, ff), dtype=torch.uint8, device=x.device)
+        saved = x.new_empty(L.scao_gated_ff_saved_bytes(rows, ff) >> 1)     # 16-bit places
     if rows:
         ins, copied = _operands((x, w_gate, w_up))
         args = _ARGS.pack(ins[0][1], ins[1][1], ins[2][1], h.data_ptr(), saved.data_ptr() if train else 0,
@@ -79,16 +79,14 @@ def _forward(x, w_gate, w_up, act, train):
 def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w, copies=None):
     """(dx, dw_gate, dw_up), None where not needed."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
-    like = dict(dtype=x.dtype, device=x.device)
-    dx = torch.empty((rows, d), **like) if need_x else None
-    new = torch.empty if rows else torch.zeros
-    dwg, dwu = (new((ff, d), **like), new((ff, d), **like)) if need_w else (None, None)
+    dx = x.new_empty((rows, d)) if need_x else None
+    new = x.new_empty if rows else x.new_zeros
+    dwg, dwu = (new((ff, d)), new((ff, d))) if need_w else (None, None)
     if rows:
         ins, _ = _operands(copies or (x, w_gate, w_up))
         if dh.stride(1) != 1:
             dh = dh.contiguous()
-        ws = torch.empty(L.scao_gated_ff_workspace_bytes(rows, d, ff, need_x | need_w << 1), dtype=torch.uint8,
-                         device=x.device)
+        ws = x.new_empty((L.scao_gated_ff_workspace_bytes(rows, d, ff, need_x | need_w << 1) + 1) >> 1)
         at = [0 if t is None else t.data_ptr() for t in (dx, dwg, dwu)]
         args = _ARGS.pack(ins[0][1], ins[1][1], ins[2][1], 0, saved.data_ptr(), dh.data_ptr(), *at,
                           ws.data_ptr(), ins[0][2], ins[1][2], ins[2][2], dh.stride(0),
