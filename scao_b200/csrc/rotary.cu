@@ -5,15 +5,19 @@
 // with (a, b) = (2j, 2j + 1) or (j, j + dim/2); values beyond dim pass through.
 // The gradient is the transposed rotation: the same kernel with -sin.
 //
-// The angle is kept in turns and in 64 bits until its whole turns are taken
-// off (p w_j / 2 pi reaches 1e5 and more, where 32 bits would leave an error of
-// 1e-2 turns); the remainder, below half a turn, goes to sincospif.  The
-// frequencies travel as kernel arguments (dim <= 512: 2 KB), so there is no
-// table in memory to keep or to outgrow.
+// The angle is formed in turns, as a fixed-point fraction of 64 bits: p times the
+// fraction w_j / 2 pi 2^64, of which a 64-bit product keeps exactly what is left when whole
+// turns are taken off (in 32-bit floats p w_j / 2 pi of far positions would be off by 1e-2
+// turns and more; doubles would do, at three conversions of a quarter of the rate
+// each).  Its upper 32 bits, as a signed part of a turn, go to sincospif.  The
+// frequencies travel as kernel arguments (dim <= 512: 2 KB), so there is no table in
+// memory to keep or to outgrow.
 //
 // A block takes a few tokens: it forms their cosines and sines once into shared
 // memory and applies them to every head of q and of k, each value read and
 // written once with the widest vector that the strides allow.  HBM bound.
+#include <math.h>
+
 #include "common.cuh"
 #include "prof.cuh"
 #include "tmap.cuh"
@@ -22,10 +26,10 @@ namespace {
 
 constexpr int RT = 256;                 // threads per block, at most
 constexpr int RMAX = 256;               // frequencies
-constexpr int RTOK = 16;                // tokens per block, at most
+constexpr int RTOK = 64;                // tokens per block, at most
 
 struct RotArgs {
-    double turn[RMAX];                  // turns per position
+    uint64_t turn[RMAX];                // turns per position, of 2^-64
     const void* in[2];
     void* out[2];
     int64_t isb[2], ish[2], ist[2], osb[2], osh[2], ost[2];   // strides in values
@@ -33,6 +37,7 @@ struct RotArgs {
     int64_t pos_sb, pos_st, start, tokens;
     int heads[2];
     int pos64, T, D, half, tb;
+    uint32_t inv_half;                  // 2^32 / half, rounded up: i / half for i < 2^14
     float cosm, sinm;                   // m and +-m
 };
 static_assert(sizeof(RotArgs) <= 4096, "kernel arguments");
@@ -71,77 +76,112 @@ union Pack {
 
 // Item of a thread, one of S per head: NV pairs of two vectors (halves apart),
 // NV / 2 pairs of one vector (interleaved; one pair where NV is 1), or a
-// vector behind the rotated part.
+// vector behind the rotated part.  A thread keeps its item and goes over (token, head)
+// rows, RROWS at a time with all their loads first; the first rows are on their way
+// while the block forms its cosines and sines.
 template <int DT, bool INTER, int NV>
 __global__ void __launch_bounds__(RT)
 rotary_kernel(const __grid_constant__ RotArgs A) {
     typedef typename ElemOf<DT>::type E;
     typedef Pack<DT, NV> V;
-    extern __shared__ float2 cs[];      // [token][pair]: m cos, +-m sin
-    const int half = A.half;
+    typedef decltype(V::v) Word;
+    constexpr bool TWO = !INTER || NV == 1;                       // a rotating item is two vectors
+    constexpr int PAIRS = INTER ? (NV > 1 ? NV / 2 : 1) : NV;     // its pairs
+    constexpr int RROWS = TWO && sizeof(Word) == 16 ? 2 : 4;
+    // m cos, +-m sin of [token][two pairs of an item][item][2]: neighbouring items read
+    // neighbouring 16 bytes (by pair, their reads met in the same banks)
+    extern __shared__ float4 cs4[];
+    float2* cs = (float2*)cs4;
+    __shared__ int64_t base[RTOK][5];   // of the token in q, k, the results and the positions
+    const int half = A.half, bx = blockDim.x, by = blockDim.y;
     const int64_t tok0 = (int64_t)blockIdx.x * A.tb;
     const int nt = (int)min((int64_t)A.tb, A.tokens - tok0);
-    const int tid = threadIdx.y * blockDim.x + threadIdx.x, nthr = blockDim.x * blockDim.y;
-    for (int i = tid; i < nt * half; i += nthr) {
-        const int k = i / half, j = i - k * half;
-        const int64_t b = (tok0 + k) / A.T, t = (tok0 + k) - b * A.T;
-        int64_t p = A.start + t;
-        if (A.pos) {
-            const int64_t o = b * A.pos_sb + t * A.pos_st;
-            p = A.pos64 ? ((const int64_t*)A.pos)[o] : (int64_t)((const int32_t*)A.pos)[o];
+    const int tid = threadIdx.y * bx + threadIdx.x, nthr = bx * by;
+    if (tid < nt) {
+        const int64_t b = (tok0 + tid) / A.T, t = (tok0 + tid) - b * A.T;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            base[tid][i] = b * A.isb[i] + t * A.ist[i];
+            base[tid][2 + i] = b * A.osb[i] + t * A.ost[i];
         }
-        const double x = (double)p * A.turn[j];
-        float s, c;
-        sincospif((float)(2.0 * (x - rint(x))), &s, &c);
-        cs[i] = make_float2(A.cosm * c, A.sinm * s);
+        base[tid][4] = A.pos ? b * A.pos_sb + t * A.pos_st : A.start + t;
     }
     __syncthreads();
-    constexpr int PAIRS = INTER ? (NV > 1 ? NV / 2 : 1) : NV;     // pairs of a rotating item
     const int rot = half / PAIRS, S = rot + (A.D - 2 * half) / NV;
-    const int H = A.heads[0] + A.heads[1], rows = nt * H;
-    for (int s = threadIdx.x; s < S; s += blockDim.x) {
+    const int H0 = A.heads[0], H = H0 + A.heads[1], rows = nt * H;
+    const int ob = INTER ? 1 : half;                              // to an item's second vector
+    int s = threadIdx.x, r = threadIdx.y, k = 0, h = threadIdx.y; // item; row, its token and head
+    V a[RROWS], x2[RROWS];
+    E* out[RROWS];
+    int tok[RROWS];
+    auto load = [&] {
         const bool turns = s < rot;
-        const int j = s * PAIRS;
-        const int oa = turns ? (INTER ? 2 * j : j) : 2 * half + (s - rot) * NV;
-        for (int r = threadIdx.y; r < rows; r += blockDim.y) {
-            const int k = r / H;
-            int h = r - k * H;
-            const int w = h >= A.heads[0];
-            if (w) h -= A.heads[0];
-            const int64_t b = (tok0 + k) / A.T, t = (tok0 + k) - b * A.T;
-            const E* in = (const E*)A.in[w] + b * A.isb[w] + h * A.ish[w] + t * A.ist[w] + oa;
-            E* out = (E*)A.out[w] + b * A.osb[w] + h * A.osh[w] + t * A.ost[w] + oa;
-            V a, y;
-            a.v = *(const decltype(a.v)*)in;
-            if (!turns) {
-                *(decltype(a.v)*)out = a.v;
+        const int oa = turns ? (INTER ? 2 : 1) * s * PAIRS : 2 * half + (s - rot) * NV;
+#pragma unroll
+        for (int u = 0; u < RROWS; ++u) {
+            tok[u] = -1;
+            if (r < rows) {
+                while (h >= H) { h -= H; ++k; }
+                const int w = h >= H0, hh = w ? h - H0 : h;
+                const E* in = (const E*)A.in[w] + base[k][w] + hh * A.ish[w] + oa;
+                out[u] = (E*)A.out[w] + base[k][2 + w] + hh * A.osh[w] + oa;
+                a[u].v = *(const Word*)in;
+                if (TWO && turns) x2[u].v = *(const Word*)(in + ob);
+                tok[u] = k;
+            }
+            r += by;
+            h += by;
+        }
+    };
+    load();
+    for (int i = tid; i < nt * half; i += nthr) {
+        const int t = half > 1 ? (int)__umulhi((uint32_t)i, A.inv_half) : i, j = i - t * half;
+        int64_t p = base[t][4];
+        if (A.pos) p = A.pos64 ? ((const int64_t*)A.pos)[p] : (int64_t)((const int32_t*)A.pos)[p];
+        const int part = (int)(((uint64_t)p * A.turn[j]) >> 32);      // of a turn, times 2^32
+        float sn, c;
+        sincospif((float)part * 0x1p-31f, &sn, &c);
+        const int item = j / PAIRS, e = j % PAIRS;
+        cs[t * half + (PAIRS > 1 ? ((e >> 1) * rot + item) * 2 + (e & 1) : item)] =
+            make_float2(A.cosm * c, A.sinm * sn);
+    }
+    __syncthreads();
+    for (;;) {
+#pragma unroll
+        for (int u = 0; u < RROWS; ++u) {
+            if (tok[u] < 0) break;
+            if (s >= rot) {
+                *(Word*)out[u] = a[u].v;
                 continue;
             }
-            const float2* c = cs + k * half + j;
-            if constexpr (INTER && NV > 1) {
+            const float2* c = cs + tok[u] * half;
+            V y, y2;
+            float4 two;
 #pragma unroll
-                for (int e = 0; e < PAIRS; ++e) {
-                    const float2 q = c[e];
-                    const float xa = to_f<DT>(a.e[2 * e]), xb = to_f<DT>(a.e[2 * e + 1]);
-                    y.e[2 * e] = from_f<DT>(xa * q.x - xb * q.y);
-                    y.e[2 * e + 1] = from_f<DT>(xa * q.y + xb * q.x);
+            for (int e = 0; e < PAIRS; ++e) {
+                if (PAIRS > 1 && e % 2 == 0) two = *(const float4*)(c + (e / 2 * rot + s) * 2);
+                const float2 q = PAIRS == 1 ? c[s] : e % 2 ? make_float2(two.z, two.w) : make_float2(two.x, two.y);
+                const float xa = to_f<DT>(TWO ? a[u].e[e] : a[u].e[2 * e % NV]);
+                const float xb = to_f<DT>(TWO ? x2[u].e[e] : a[u].e[(2 * e + 1) % NV]);
+                const E ya = from_f<DT>(xa * q.x - xb * q.y), yb = from_f<DT>(xa * q.y + xb * q.x);
+                if (TWO) {
+                    y.e[e] = ya;
+                    y2.e[e] = yb;
+                } else {
+                    y.e[2 * e % NV] = ya;
+                    y.e[(2 * e + 1) % NV] = yb;
                 }
-                *(decltype(a.v)*)out = y.v;
-            } else {
-                const int ob = INTER ? 1 : half;
-                V x2, y2;
-                x2.v = *(const decltype(a.v)*)(in + ob);
-#pragma unroll
-                for (int e = 0; e < NV; ++e) {
-                    const float2 q = c[e];
-                    const float xa = to_f<DT>(a.e[e]), xb = to_f<DT>(x2.e[e]);
-                    y.e[e] = from_f<DT>(xa * q.x - xb * q.y);
-                    y2.e[e] = from_f<DT>(xa * q.y + xb * q.x);
-                }
-                *(decltype(a.v)*)out = y.v;
-                *(decltype(a.v)*)(out + ob) = y2.v;
             }
+            *(Word*)out[u] = y.v;
+            if (TWO) *(Word*)(out[u] + ob) = y2.v;
         }
+        if (r >= rows) {                                          // the next item
+            s += bx;
+            r = h = threadIdx.y;
+            k = 0;
+        }
+        if (s >= S) break;
+        load();
     }
 }
 
@@ -150,11 +190,13 @@ int launch(RotArgs& A, cudaStream_t st) {
     constexpr int PAIRS = INTER ? (NV > 1 ? NV / 2 : 1) : NV;
     const int S = A.half / PAIRS + (A.D - 2 * A.half) / NV, H = A.heads[0] + A.heads[1];
     const int bx = S < RT ? S : RT, by = RT / bx;
-    // about four rows a thread, unless that would leave SMs without a block
-    int64_t tb = (4 * by + H - 1) / H;
+    // up to four rows a thread, unless that would leave SMs without a block (eight, or a row
+    // beyond four, took 10 to 20 % longer)
+    int64_t tb = 4 * by / H;
     const int64_t spread = A.tokens / (2 * scao_sm_count());
     if (tb > spread) tb = spread;
     if (tb > RTOK) tb = RTOK;
+    if (tb > 4096 / A.half) tb = 4096 / A.half;                   // 32 KB of cosines and sines
     if (tb < 1) tb = 1;
     A.tb = (int)tb;
     const int64_t grid = (A.tokens + tb - 1) / tb;
@@ -199,7 +241,12 @@ extern "C" int scao_rotary(const ScaoRotary* r, void* stream) {
     A.cosm = r->factor;
     A.sinm = r->inverse ? -r->factor : r->factor;
     const int es = r->dtype == SCAO_F32 ? 4 : 2;
-    for (int j = 0; j < A.half; ++j) A.turn[j] = r->turns[j];
+    A.inv_half = (uint32_t)((0x100000000ull + A.half - 1) / A.half);
+    for (int j = 0; j < A.half; ++j) {
+        const double whole = floor(r->turns[j]), x = ldexp(r->turns[j] - whole, 64);
+        if (!(x >= 0)) return SCAO_ERR_ARG;             // not a number, infinite
+        A.turn[j] = x >= 0x1p64 ? 0 : (uint64_t)x;
+    }
     // widest vector that every address, stride and part of the head allows
     int64_t bits = A.D | (r->interleaved ? r->dim : A.half);
     for (int i = 0; i < 2; ++i) {
