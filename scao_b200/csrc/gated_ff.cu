@@ -645,16 +645,14 @@ ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict_
     }
 }
 
-// Few rows (at most SK_ROWS): the time is one reading of the weights, so no tile
-// waits for a whole operand block.  A warp takes 8 inner columns: the 16 rows of an
-// mma.m16n8k16 A operand are their 8 gate and 8 up weight rows, loaded straight
-// from global memory into the registers that the instruction reads (a contraction
-// may take its terms in any order, so a lane's 16 consecutive bytes serve as the
-// k places of two instructions, in x as in the weights).  Gate and up of one place
-// meet in one thread.  The block's warps share a row's contraction and join in
-// shared memory in a fixed order.
-constexpr int SK_WARPS = 8;
-constexpr int SK_ROWS = 32;
+// Few rows: the time is one reading of the weights, so no tile waits for a whole
+// operand block.  A warp takes 8 FG inner columns: the 16 rows of an mma.m16n8k16 A
+// operand are 8 gate and 8 up weight rows, loaded straight from global memory into the
+// registers that the instruction reads (a contraction may take its terms in any order,
+// so a lane's 16 consecutive bytes serve as the k places of two instructions, in x as
+// in the weights).  Gate and up of one place meet in one thread.  The block's warps
+// share a row's contraction and join in shared memory in a fixed order.
+constexpr int SK_ROWS = 64;
 
 SCAO_DEV void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                         uint32_t b1, bool bf16) {
@@ -678,15 +676,19 @@ SCAO_DEV uint4 load8_guard(const uint16_t* p, int left) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Registers: up to 8 rows at most 72, so that seven blocks of four warps fit an SM (1024
+// blocks, the columns of 8192, are then one wave).
+constexpr int sk_registers(int nt) { return nt == 1 ? 72 : nt == 2 ? 64 : nt == 4 ? 128 : 144; }
+
 template <int ACT, bool BF16, int NT, int FG>
-__global__ void __launch_bounds__(32 * SK_WARPS)
+__global__ void __maxnreg__(sk_registers(NT))
 ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ wg, int64_t ldg,
                  const uint16_t* __restrict__ wu, int64_t ldu, uint16_t* __restrict__ h, int rows, int d,
                  int ff) {
-    constexpr int U = NT == 1 ? 4 : 2;          // 32-deep steps in flight
-    __shared__ float part[SK_WARPS][FG * NT * 4][32];
+    constexpr int U = NT == 1 ? 4 : NT <= 4 ? 2 : 1;      // 32-deep steps in flight
+    extern __shared__ float part[];                       // [warp][NT * 4][lane]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int f0 = blockIdx.x * 8 * FG + g;
+    const int warps = blockDim.x >> 5, f0 = blockIdx.x * 8 * FG + g;
     float acc[FG][NT][4];
 #pragma unroll
     for (int j = 0; j < FG; ++j)
@@ -694,7 +696,7 @@ ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[j][n][i] = 0.f;
-    for (int k0 = warp * 32 * U; k0 < d; k0 += SK_WARPS * 32 * U) {
+    for (int k0 = warp * 32 * U; k0 < d; k0 += warps * 32 * U) {
         uint4 a[FG][U], b[FG][U], v[NT][U];
 #pragma unroll
         for (int s = 0; s < U; ++s) {
@@ -723,29 +725,29 @@ ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __
                 }
     }
 #pragma unroll
-    for (int j = 0; j < FG; ++j)
+    for (int j = 0; j < FG; ++j) {
+        if (j) __syncthreads();
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[warp][(j * NT + n) * 4 + i][lane] = acc[j][n][i];
-    __syncthreads();
-    // a warp per (column group, row group); rows 2t + i, gate in place i and up in 2 + i
-    if (warp < FG * NT) {
-        const int j = warp / NT, n = warp - j * NT, f = f0 + 8 * j;
+            for (int i = 0; i < 4; ++i) part[(warp * NT * 4 + n * 4 + i) * 32 + lane] = acc[j][n][i];
+        __syncthreads();
+        // a warp per row group; rows 2t + i, gate in place i and up in 2 + i
+        const int f = f0 + 8 * j;
+        for (int n = warp; n < NT; n += warps)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float gate = 0.f, upv = 0.f;
-#pragma unroll
-            for (int w = 0; w < SK_WARPS; ++w) {
-                gate += part[w][warp * 4 + i][lane];
-                upv += part[w][warp * 4 + 2 + i][lane];
+            for (int i = 0; i < 2; ++i) {
+                float gate = 0.f, upv = 0.f;
+                for (int w = 0; w < warps; ++w) {
+                    gate += part[(w * NT * 4 + n * 4 + i) * 32 + lane];
+                    upv += part[(w * NT * 4 + n * 4 + 2 + i) * 32 + lane];
+                }
+                const int r = n * 8 + 2 * t + i;
+                if (f < ff && r < rows) {
+                    const float y = ff_act<ACT>(gate) * upv;
+                    h[(int64_t)r * ff + f] = BF16 ? f_to_bf16_bits(y) : f_to_f16_bits(y);
+                }
             }
-            const int r = n * 8 + 2 * t + i;
-            if (f < ff && r < rows) {
-                const float y = ff_act<ACT>(gate) * upv;
-                h[(int64_t)r * ff + f] = BF16 ? f_to_bf16_bits(y) : f_to_f16_bits(y);
-            }
-        }
     }
 }
 
@@ -957,6 +959,18 @@ int64_t tiles_of(int64_t rows, int64_t cols, int tm, int tn) {
     return ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn);
 }
 
+// Whether few rows go through ff_skinny_kernel: every block reads x again, so by the bytes
+// it takes in (about 8 MB a microsecond) against the tensor-core tiles' steps.  At 32 rows
+// 1024 x 4096 takes 8.5 and 12.2 us, 2048 x 8192 20.1 and 19.6.
+bool plan_skinny(int rows, int d, int ff) {
+    if (rows <= 16) return true;
+    if (rows > SK_ROWS) return false;
+    const double bytes = 4.0 * d * ff + 2.0 * up(ff, 16) * rows * d;
+    if (rows > 32 && up(ff, 16) > scao_sm_count()) return false;        // one block an SM: its registers
+    const int64_t waves = (tiles_of(rows, ff, 128, 64) + scao_sm_count() - 1) / scao_sm_count();
+    return 2.5 + bytes / 8e6 < 6.0 + step_us(SINGLE) * up(d, 64) * (double)waves;
+}
+
 int plan_forward(int rows, int ff) {
     int best = SINGLE;
     double least = 0;
@@ -1016,11 +1030,19 @@ int take_status() {
 
 template <int ACT, bool BF16>
 int launch_skinny(const ScaoGatedFf* f, cudaStream_t st) {
-    const int nt = (f->rows + 7) / 8, fg = nt > 2 ? 2 : 1;
-    auto* kernel = nt == 1 ? ff_skinny_kernel<ACT, BF16, 1, 1>
-                   : nt == 2 ? ff_skinny_kernel<ACT, BF16, 2, 1> : ff_skinny_kernel<ACT, BF16, 4, 2>;
+    const int groups = (f->rows + 7) / 8, nt = groups <= 2 ? groups : groups <= 4 ? 4 : 8;
+    const int fg = nt > 2 ? 2 : 1, blocks = up(f->ff, 8 * fg);
+    auto* kernel = nt == 1   ? ff_skinny_kernel<ACT, BF16, 1, 1>
+                   : nt == 2 ? ff_skinny_kernel<ACT, BF16, 2, 1>
+                   : nt == 4 ? ff_skinny_kernel<ACT, BF16, 4, 2> : ff_skinny_kernel<ACT, BF16, 8, 2>;
+    // Warps that share a contraction: 4 fill the SMs where the columns are many (8192 columns
+    // of 2048: 14.1 us, with 8 15.8), more where they are few (1000 of 2048: 7.2 us with 4, 4.7
+    // with 8), as far as the contraction gives each a step.
+    const int step = nt == 1 ? 128 : nt <= 4 ? 64 : 32, most = nt <= 2 ? 16 : 8;
+    int warps = 4;
+    while (warps < most && 2 * warps * blocks <= 24 * scao_sm_count() && warps * step < f->d) warps *= 2;
     ProfScope p(SLOT_GATED_FF, st);
-    kernel<<<up(f->ff, 8 * fg), 32 * SK_WARPS, 0, st>>>(
+    kernel<<<blocks, 32 * warps, (size_t)warps * nt * 4 * 32 * sizeof(float), st>>>(
         (const uint16_t*)f->x, f->ldx, (const uint16_t*)f->w_gate, f->ldg, (const uint16_t*)f->w_up, f->ldu,
         (uint16_t*)f->h, f->rows, f->d, f->ff);
     SCAO_CHECK_LAUNCH();
@@ -1096,7 +1118,7 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     if (!f->h) return SCAO_ERR_ARG;
     if (int rc = take_status()) return rc;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (!f->saved && f->rows <= SK_ROWS) {
+    if (!f->saved && plan_skinny(f->rows, f->d, f->ff)) {
         if (f->act == SCAO_ACT_SILU) return launch_skinny<SCAO_ACT_SILU>(f, st);
         if (f->act == SCAO_ACT_GELU) return launch_skinny<SCAO_ACT_GELU>(f, st);
         return launch_skinny<SCAO_ACT_GELU_TANH>(f, st);

@@ -120,9 +120,16 @@ def test_activations(m, act, train):
     check(x, wg * 4, wu, act, train)         # gates up to about 15 both ways
 
 
-@pytest.mark.parametrize("m", range(1, 41))
+@pytest.mark.parametrize("m", range(1, 70))
 def test_every_small_row_count(m):
     check(*inputs(m, 136, 72, torch.float16), "silu", False)
+
+
+@pytest.mark.parametrize("m", [1, 12, 30, 60])
+@pytest.mark.parametrize("d,f", [(33, 9000), (1100, 1000), (2500, 17), (4, 300)])
+def test_few_rows_of_other_widths(m, d, f):
+    """One to sixteen warps share a contraction; widths that leave warps without a step."""
+    check(*inputs(m, d, f, torch.bfloat16), "gelu", False)
 
 
 @pytest.mark.parametrize("m,d,f", [(2100, 320, 1500), (1500, 700, 1600), (3000, 1100, 2100), (600, 2000, 700),
