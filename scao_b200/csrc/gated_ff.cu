@@ -16,9 +16,9 @@
 //   dW         dg^T x and du^T x over the rows, both operands MN-major: nothing is
 //              transposed in memory.
 // The pointwise part of the gradient (ff_pointwise_kernel) reads g and u as the
-// forward pass kept them, in 32 bits: rounding them to 16 as well would add their
-// rounding to those of dg, du (16 bits: they are operands of the tensor cores)
-// and of the result, and put the gradients' error at 1.8 instead of 1.4 roundings.
+// forward pass kept them, in 24 bits: in 16 their rounding would come beside those
+// of dg, du (16 bits: they are operands of the tensor cores) and of the result, and
+// put the gradients' error at 1.8 instead of 1.4 roundings.
 #include <cuda.h>
 #include <string.h>
 
@@ -71,7 +71,7 @@ struct FfGemm {
     // 64 of what is read MN-major, 32 of the results (h, or dx, dWg, dWu)
     CUtensorMap x, w[2], dguk[2], dgum[2], out[3];
     FfWork work[2];                         // in the order in which a CTA (pair) takes them
-    float* saved;                           // forward: g and u for the gradient, or null
+    unsigned char* saved;                   // forward: g and u for the gradient, or null
     float* partial;                         // split tiles: sums of the items
     int* count;                             // split tiles: items done, per epilogue warp
     int* status;
@@ -161,14 +161,43 @@ SCAO_DEV uint32_t pack2(float a, float b, int dt) {
     return (uint32_t)f_to_f16_bits(a) | ((uint32_t)f_to_f16_bits(b) << 16);
 }
 
-// g and u as kept for the gradient: per 128-row x 128-column block the g values,
-// then the u values, as [4-column group][row][4], so that a warp (a thread per row)
-// writes 512 consecutive bytes.
+// g and u as kept for the gradient: rounded to 24 bits (16 of the significand), 3 bytes a
+// value, which is 2^-8 of a 16-bit rounding and a quarter less to write and read than 32.
+// Per 128-row x 128-column block the g values, then the u values, as [16-column
+// group][16 bytes of its 48][row], so that a warp (a thread per row) writes 512
+// consecutive bytes.
+constexpr int SAVED_BLOCK = 128 * 128 * 3;
 SCAO_DEV int64_t saved_off(int row, int col, int col_blocks) {
-    return ((int64_t)(row >> 7) * col_blocks + (col >> 7)) * (2 * 128 * 128) +
-           (((col & 127) >> 2) * 128 + (row & 127)) * 4;
+    return ((int64_t)(row >> 7) * col_blocks + (col >> 7)) * (2 * SAVED_BLOCK) +
+           (((col & 127) >> 4) * 3 * 128 + (row & 127)) * 16;
 }
-constexpr int SAVED_U = 128 * 128;
+constexpr int SAVED_PLANE = 128 * 16;
+
+// to nearest, ties away; infinities and NaN as they are
+SCAO_DEV uint32_t round24(uint32_t x) { return (x & 0x7fffffffu) < 0x7f800000u ? x + 0x80u : x; }
+
+SCAO_DEV void save16(unsigned char* p, const uint32_t* v) {
+    uint32_t w[12];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = round24(v[4 * i]), b = round24(v[4 * i + 1]), c = round24(v[4 * i + 2]),
+                       d = round24(v[4 * i + 3]);
+        w[3 * i] = __byte_perm(a, b, 0x5321);           // upper three bytes of each, in turn
+        w[3 * i + 1] = __byte_perm(b, c, 0x6532);
+        w[3 * i + 2] = __byte_perm(c, d, 0x7653);
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+        *(uint4*)(p + i * SAVED_PLANE) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
+// the four values of three of those words
+SCAO_DEV void restore4(uint32_t w0, uint32_t w1, uint32_t w2, float* v) {
+    v[0] = __uint_as_float(w0 << 8);
+    v[1] = __uint_as_float(__byte_perm(w0, w1, 0x5433) & 0xffffff00u);
+    v[2] = __uint_as_float(__byte_perm(w1, w2, 0x4322) & 0xffffff00u);
+    v[3] = __uint_as_float(w2 & 0xffffff00u);
+}
 
 SCAO_DEV void ff_fail(int* status) { *(volatile int*)status = 2; }
 
@@ -477,12 +506,9 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
                 for (int c = 0; c < 64; c += 16) {
                     const uint32_t *g = gr + c, *u = ur + c;
                     if (G.saved && row < w.rows && c0 + c < w.cols) {
-                        float* p = G.saved + saved_off(row, c0 + c, cb);
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            *(uint4*)(p + i * 128) = make_uint4(g[i], g[i + 1], g[i + 2], g[i + 3]);
-                            *(uint4*)(p + SAVED_U + i * 128) = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
-                        }
+                        unsigned char* p = G.saved + saved_off(row, c0 + c, cb);
+                        save16(p, g);
+                        save16(p + SAVED_BLOCK, u);
                     }
                     float y[16];
 #pragma unroll
@@ -586,14 +612,14 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
 }
 
 // dg = dh u act'(g), du = dh act(g).  A block takes `span` rows of a 128-column block of
-// g and u as they were kept; a warp 8 rows x 16 columns at a time: runs of 128 bytes of g and u and
-// of 32 of the others.  HBM bound (14 bytes a value): 4096 x 8192 in PW_US us, a copy of
-// as many bytes takes 77.  (4 rows x 32 columns took 90, 2 x 64 94, 1 x 128 111 us.)
+// g and u as they were kept; a warp 8 rows x 64 columns at a time, a thread 16 columns
+// of a row: runs of 128 bytes of every array.  HBM bound (12 bytes a value): 4096 x 8192 in
+// PW_US us.
 constexpr int PT = 256;
 
 template <int ACT>
-__global__ void __launch_bounds__(PT, 4)
-ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict__ dh, int64_t lddh,
+__global__ void __launch_bounds__(PT)
+ff_pointwise_kernel(const unsigned char* __restrict__ saved, const uint16_t* __restrict__ dh, int64_t lddh,
                     uint16_t* __restrict__ dg, uint16_t* __restrict__ du, int64_t ldg, int rows,
                     int cols, int dtype, int vec, int span, int* count, int n_count) {
     tc_grid_release();                      // the products may set up while this runs
@@ -602,45 +628,61 @@ ff_pointwise_kernel(const float* __restrict__ saved, const uint16_t* __restrict_
          i += gridDim.x * gridDim.y * PT)
         count[i] = 0;
     const int cb = (cols + 127) >> 7, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c = blockIdx.y * 128 + warp * 16 + (lane & 3) * 4;
+    const int c = blockIdx.y * 128 + (warp & 1) * 64 + (lane & 3) * 16;
     if (c >= cols) return;
-    const int r0 = blockIdx.x * span + (lane >> 2);
-#pragma unroll 1
-    for (int i = 0; i < span; i += 16) {
-        if (r0 + i >= rows) break;
-        float4 g[2], u[2], y[2];
+    for (int i = (warp >> 1) * 8 + (lane >> 2); i < span; i += 32) {
+        const int r = blockIdx.x * span + i;
+        if (r >= rows) break;
+        const unsigned char* p = saved + saved_off(r, c, cb);
+        uint4 gw[3], uw[3];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {                   // all loads first
-            const int r = min(r0 + i + 8 * k, rows - 1);
-            const float* p = saved + saved_off(r, c, cb);
-            g[k] = *(const float4*)p;
-            u[k] = *(const float4*)(p + SAVED_U);
-            const uint16_t* d = dh + r * lddh + c;
-            if (vec) {
-                y[k] = load4_dt(d, 0, dtype);
-            } else {
-                y[k].x = load_dt(d, 0, dtype);
-                y[k].y = c + 1 < cols ? load_dt(d, 1, dtype) : 0.f;
-                y[k].z = c + 2 < cols ? load_dt(d, 2, dtype) : 0.f;
-                y[k].w = c + 3 < cols ? load_dt(d, 3, dtype) : 0.f;
+        for (int k = 0; k < 3; ++k) {
+            gw[k] = *(const uint4*)(p + k * SAVED_PLANE);
+            uw[k] = *(const uint4*)(p + SAVED_BLOCK + k * SAVED_PLANE);
+        }
+        const uint16_t* d = dh + r * lddh + c;
+        uint32_t y[8];
+        if (vec) {
+            const bool all = c + 8 < cols;
+            const uint4 a = *(const uint4*)d, b = all ? *(const uint4*)(d + 8) : make_uint4(0, 0, 0, 0);
+            y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w;
+            y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                y[k] = (c + 2 * k < cols ? (uint32_t)d[2 * k] : 0) |
+                       (c + 2 * k + 1 < cols ? (uint32_t)d[2 * k + 1] << 16 : 0);
+        }
+        const uint32_t gq[12] = {gw[0].x, gw[0].y, gw[0].z, gw[0].w, gw[1].x, gw[1].y,
+                                 gw[1].z, gw[1].w, gw[2].x, gw[2].y, gw[2].z, gw[2].w};
+        const uint32_t uq[12] = {uw[0].x, uw[0].y, uw[0].z, uw[0].w, uw[1].x, uw[1].y,
+                                 uw[1].z, uw[1].w, uw[2].x, uw[2].y, uw[2].z, uw[2].w};
+        uint32_t og[8], ou[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float g[4], u[4], a[4], b[4], z[4];
+            restore4(gq[3 * k], gq[3 * k + 1], gq[3 * k + 2], g);
+            restore4(uq[3 * k], uq[3 * k + 1], uq[3 * k + 2], u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t bits = y[2 * k + (e >> 1)] >> (16 * (e & 1)) & 0xffff;
+                z[e] = dtype == SCAO_BF16 ? bf16_bits_to_f(bits) : f16_bits_to_f(bits);
+                ff_act_grad<ACT>(g[e], a[e], b[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                ou[2 * k + e / 2] = pack2(z[e] * a[e], z[e + 1] * a[e + 1], dtype);
+                og[2 * k + e / 2] = pack2(z[e] * u[e] * b[e], z[e + 1] * u[e + 1] * b[e + 1], dtype);
             }
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int r = r0 + i + 8 * k;
-            if (r >= rows) break;
-            float4 a, b;
-            ff_act_grad<ACT>(g[k].x, a.x, b.x);
-            ff_act_grad<ACT>(g[k].y, a.y, b.y);
-            ff_act_grad<ACT>(g[k].z, a.z, b.z);
-            ff_act_grad<ACT>(g[k].w, a.w, b.w);
-            const float4 d = y[k];
-            // the pitch of dg and du is a multiple of 8: the last group may write past
-            // `cols` within it, where the products read nothing
-            store4_dt(du + r * ldg + c, 0, dtype, make_float4(d.x * a.x, d.y * a.y, d.z * a.z, d.w * a.w));
-            store4_dt(dg + r * ldg + c, 0, dtype,
-                      make_float4(d.x * u[k].x * b.x, d.y * u[k].y * b.y, d.z * u[k].z * b.z,
-                                  d.w * u[k].w * b.w));
+        // the pitch of dg and du is a multiple of 8: a half may write past `cols` within it,
+        // where the products read nothing
+        uint16_t *pg = dg + r * ldg + c, *pu = du + r * ldg + c;
+        *(uint4*)pg = make_uint4(og[0], og[1], og[2], og[3]);
+        *(uint4*)pu = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+        if (c + 8 < ldg) {
+            *(uint4*)(pg + 8) = make_uint4(og[4], og[5], og[6], og[7]);
+            *(uint4*)(pu + 8) = make_uint4(ou[4], ou[5], ou[6], ou[7]);
         }
     }
 }
@@ -1078,7 +1120,7 @@ bool operands_ok(const ScaoGatedFf* f) {
 extern "C" int* scao_gated_ff_status_word(void) { return status_word(); }
 
 extern "C" int64_t scao_gated_ff_saved_bytes(int rows, int ff) {
-    return (int64_t)up(rows, 128) * up(ff, 128) * (2 * 128 * 128) * (int64_t)sizeof(float);
+    return (int64_t)up(rows, 128) * up(ff, 128) * (2 * SAVED_BLOCK);
 }
 
 extern "C" int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff, int which) {
@@ -1143,7 +1185,7 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
         !map_operand(&G.w[1], f->w_up, f->ff, f->d, f->ldu, f->dtype, box) ||
         (w.tma_out && !map_result(&G.out[0], f->h, f->rows, f->ff, f->dtype)))
         return SCAO_ERR_LAUNCH;
-    G.saved = (float*)f->saved;
+    G.saved = (unsigned char*)f->saved;
     G.status = status_word();
     G.dtype = f->dtype;
     const int n = (int)items;
@@ -1167,16 +1209,16 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
     char* ws = (char*)f->workspace;
     uint16_t *dg = (uint16_t*)ws, *du = (uint16_t*)(ws + space.du);
     {
-        const int vec = ((uintptr_t)f->dh & 7) == 0 && (f->lddh & 3) == 0 && (f->ff & 3) == 0;
+        const int vec = ((uintptr_t)f->dh & 15) == 0 && (f->lddh & 7) == 0 && (f->ff & 7) == 0;
         ProfScope prof(SLOT_GATED_FF, st);
         auto* kernel = f->act == SCAO_ACT_SILU   ? ff_pointwise_kernel<SCAO_ACT_SILU>
                        : f->act == SCAO_ACT_GELU ? ff_pointwise_kernel<SCAO_ACT_GELU>
                                                  : ff_pointwise_kernel<SCAO_ACT_GELU_TANH>;
         // rows of a block: 128, fewer where that would leave SMs without one
         int span = 128;
-        while (span > 16 && (int64_t)up(f->rows, span) * up(f->ff, 128) < 4 * scao_sm_count()) span >>= 1;
+        while (span > 32 && (int64_t)up(f->rows, span) * up(f->ff, 128) < 4 * scao_sm_count()) span >>= 1;
         kernel<<<dim3(up(f->rows, span), up(f->ff, 128)), PT, 0, st>>>(
-            (const float*)f->saved, (const uint16_t*)f->dh, f->lddh, dg, du, ld, f->rows, f->ff, f->dtype, vec,
+            (const unsigned char*)f->saved, (const uint16_t*)f->dh, f->lddh, dg, du, ld, f->rows, f->ff, f->dtype, vec,
             span, (int*)(ws + space.count), (int)p.counts);
         SCAO_CHECK_LAUNCH();
     }

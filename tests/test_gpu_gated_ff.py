@@ -5,7 +5,8 @@ them is off by at most n 2^-23 (tensor cores may cut instead of round) of the su
 magnitudes: E below, carried through the activation, whose derivative is below 1.2
 and whose own error in 32 bits is below 2^-19 of its argument's size.  Each rounding to
 the type adds half a step (r = eps / 2): one for h, one for dg and du (operands) and one
-for the gradients.
+for the gradients, which read g and u rounded to 24 bits (16 of the significand): K = 2^-16
+of each.
 """
 import math
 
@@ -17,6 +18,7 @@ from scao_b200 import GatedFeedForward, _lib, gated_ff, gpt
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 T = {"bf16": torch.bfloat16, "f16": torch.float16}
+K = 2.0 ** -16
 ACTS = ["silu", "gelu", "gelu_tanh"]
 
 
@@ -61,7 +63,9 @@ def backward64(x, wg, wu, dh, kind):
     with torch.enable_grad():
         (d,) = torch.autograd.grad(act64(gr, kind).sum(), [gr])
     dg, du = dh * u * d, dh * a
+    eg, eu = eg + K * g.abs(), eu + K * u.abs()
     ed = 1.2 * eg + 2.0 ** -19 * (1 + g.abs())        # act'' is below 1.2
+    ea = 1.2 * eg + 2.0 ** -19 * g.abs()
     edg = dh.abs() * (eu * d.abs() + ed * u.abs() + ed * eu)
     edu = dh.abs() * ea
     edg, edu = edg * (1 + r) + r * dg.abs() + tiny(t), edu * (1 + r) + r * du.abs() + tiny(t)
