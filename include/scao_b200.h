@@ -463,7 +463,7 @@ SCAO_API int scao_rotary(const ScaoRotary* args, void* stream);
  * of scao_gated_ff_workspace_bytes (which: 1 dx, 2 dw, 3 both), 16-byte
  * aligned.  pack: copies up to three matrices, rows {source, copy, rows,
  * columns, source row pitch} of the host table, to the next row pitch that
- * is a multiple of 8 values, zeros behind each row; copies start on 16
+ * is a multiple of 64 values, zeros behind each row; copies start on 16
  * bytes.  A kernel whose wait
  * ran out sets the status word (host memory; null where there is no GPU);
  * the next call clears it and returns SCAO_ERR_TIMEOUT without launching.  */

@@ -239,19 +239,29 @@ SCAO_DEV void ff_store_block(const FfWork& w, const CUtensorMap* map, int part, 
     } else {
         // an odd pitch: every other row begins between two 32-bit words, and a lane's
         // word is then the upper half of its pair and the lower half of the next lane's
-#pragma unroll 4
-        for (int r = 0; r < 32; ++r) {
-            uint16_t* d = out + (row0 + r) * w.ldo;
-            const int odd = ((uintptr_t)d >> 1) & 1, c = 2 * lane + odd;
-            uint32_t x = *(const uint32_t*)at(r, 2 * lane);
+        uint16_t* d = out + row0 * w.ldo;
+        auto even = [&](int r) {
+            const uint32_t x = *(const uint32_t*)at(r, 2 * lane);
+            uint16_t* p = d + r * w.ldo + 2 * lane;
+            if (r >= rows) return;
+            if (2 * lane + 1 < cols) *(uint32_t*)p = x;
+            else if (2 * lane < cols) *p = (uint16_t)x;
+        };
+        auto odd = [&](int r) {
+            const uint32_t x = *(const uint32_t*)at(r, 2 * lane);
             const uint32_t next = __shfl_down_sync(0xffffffffu, x, 1);
-            if (r >= rows) continue;
-            if (odd) {
-                if (lane == 0 && cols > 0) d[0] = (uint16_t)x;
-                x = __funnelshift_r(x, next, 16);
-            }
-            if (c + 1 < cols) *(uint32_t*)(d + c) = x;
-            else if (c < cols) d[c] = (uint16_t)x;
+            uint16_t* p = d + r * w.ldo + 2 * lane + 1;
+            if (r >= rows) return;
+            if (lane < 31 && 2 * lane + 2 < cols) *(uint32_t*)p = __funnelshift_r(x, next, 16);
+            else if (2 * lane + 1 < cols) *p = (uint16_t)(x >> 16);
+            if (lane == 0 && cols > 0) p[-1] = (uint16_t)x;
+        };
+        if ((uintptr_t)d & 2) {
+#pragma unroll 4
+            for (int r = 0; r < 32; r += 2) { odd(r); even(r + 1); }
+        } else {
+#pragma unroll 4
+            for (int r = 0; r < 32; r += 2) { even(r); odd(r + 1); }
         }
     }
     __syncwarp();
@@ -675,15 +685,13 @@ ff_pointwise_kernel(const unsigned char* __restrict__ saved, const uint16_t* __r
                 og[2 * k + e / 2] = pack2(z[e] * u[e] * b[e], z[e + 1] * u[e + 1] * b[e + 1], dtype);
             }
         }
-        // the pitch of dg and du is a multiple of 8: a half may write past `cols` within it,
-        // where the products read nothing
+        // dg and du have a pitch of whole lines: this may write past `cols` within it, where the
+        // products read nothing
         uint16_t *pg = dg + r * ldg + c, *pu = du + r * ldg + c;
         *(uint4*)pg = make_uint4(og[0], og[1], og[2], og[3]);
+        *(uint4*)(pg + 8) = make_uint4(og[4], og[5], og[6], og[7]);
         *(uint4*)pu = make_uint4(ou[0], ou[1], ou[2], ou[3]);
-        if (c + 8 < ldg) {
-            *(uint4*)(pg + 8) = make_uint4(og[4], og[5], og[6], og[7]);
-            *(uint4*)(pu + 8) = make_uint4(ou[4], ou[5], ou[6], ou[7]);
-        }
+        *(uint4*)(pu + 8) = make_uint4(ou[4], ou[5], ou[6], ou[7]);
     }
 }
 
@@ -793,9 +801,9 @@ ff_skinny_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __
     }
 }
 
-// Copies of operands whose rows TMA cannot read, at the next pitch that is a multiple of
-// 8 values, zeros behind each row: up to three matrices in one launch, a thread per 16
-// bytes written.  Where the two 16-byte words around a source run lie inside the
+// Copies of operands whose rows TMA cannot read, at a pitch of whole 128-byte lines (a
+// tile's rows at 16-byte steps cost a fifth sector for every four), zeros behind each row:
+// up to three matrices in one launch, a thread per 16 bytes written.  Where the two 16-byte words around a source run lie inside the
 // matrix they are loaded whole and shifted, else (its first and last few values) by
 // single values.
 struct FfPack {
@@ -811,19 +819,21 @@ ff_pack_kernel(const __grid_constant__ FfPack P) {
     int m = 0;
     while (m < P.n && i >= P.vecs[m]) i -= P.vecs[m++];
     if (m == P.n) return;
-    const int cols = P.cols[m], per = (cols + 7) >> 3;
+    const int cols = P.cols[m], per = (cols + 63) >> 6 << 3;
     const int64_t row = i / per;
     const int c = (int)(i - row * per) * 8, left = cols - c;
     const uint16_t* p = P.src[m] + row * P.pitch[m] + c;
     const uint16_t* end = P.src[m] + (P.rows[m] - 1) * P.pitch[m] + cols;
     const int off = (int)((uintptr_t)p & 15);
     const uint16_t* lo = p - off / 2;
-    uint4 y;
-    if (off == 0 && left >= 8) {
-        y = *(const uint4*)p;
-    } else if (lo >= P.src[m] && lo + 16 <= end) {
+    uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (left >= 8 && off == 0) {
+        const uint4 a = *(const uint4*)p;
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    } else if (left > 0 && lo >= P.src[m] && lo + 16 <= end) {
         const uint4 a = *(const uint4*)lo, b = *(const uint4*)(lo + 8);
-        uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
         if (off & 8)
 #pragma unroll
             for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
@@ -836,21 +846,18 @@ ff_pack_kernel(const __grid_constant__ FfPack P) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)         // nothing behind the row
             if (2 * k + 1 >= left) w[k] = 2 * k < left ? w[k] & 0xffff : 0;
-        y = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-        uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             if (k < left) w[k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
-        y = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *(uint4*)(P.dst[m] + (row * per) * 8 + c) = y;
+    *(uint4*)(P.dst[m] + (row * per) * 8 + c) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+int64_t up64(int64_t n) { return (n + 63) / 64 * 64; }
 int up(int64_t n, int k) { return (int)((n + k - 1) / k); }
 
 template <int SHAPE, bool FORWARD, int ACT>
@@ -905,12 +912,16 @@ int64_t longest(int64_t na, int64_t la, int64_t nb, int64_t lb, int extra, int G
     return x > y ? x : y;
 }
 
-// Microseconds of a step of a tile.  A CTA takes in about 50 bytes of operands a clock,
-// whatever the shape: the 32 KB of SINGLE and PAIR bound their steps (the tensor cores
-// need 256 and 512 clocks of them), the 48 KB of TALL take about its 1024 clocks.
+// Microseconds, measured, of which the plan is chosen.  A step of a tile: a CTA takes in
+// about 50 bytes of operands a clock, whatever the shape, so the 32 KB of SINGLE and PAIR
+// bound their steps (the tensor cores need 256 and 512 clocks of them), the 48 KB of TALL
+// take about its 1024 clocks.  Set-up, first copies and the last epilogue, beyond SINGLE's.
+// Joining a tile's shares.
 double step_us(int shape) { return shape == SINGLE ? 0.35 : shape == PAIR ? 0.40 : 0.72; }
-// and of joining a tile's shares
-double join_us(int shape, int splits) { return splits > 1 ? 1.5 + 0.3 * splits * (shape == PAIR ? 2 : 1) : 0; }
+double begin_us(int shape) { return shape == SINGLE ? 0.0 : shape == PAIR ? 1.2 : 1.6; }
+double join_us(int shape, int splits) {
+    return splits == 1 ? 0.0 : shape == SINGLE ? 1.5 + 0.3 * splits : 4.0 + 1.0 * splits;
+}
 
 struct FfPlan {
     int shape;
@@ -967,7 +978,7 @@ FfPlan plan_shape(int shape, int rows, int d, int ff, int dx_splits, int dw_spli
     const int a = p.dx_first ? lx : lw, b = p.dx_first ? lw : lx;
     p.extra = b ? (a + b / 2) / b : 0;
     const int most = p.dx.splits > p.dw.splits ? p.dx.splits : p.dw.splits;
-    p.us = join_us(shape, most) + step_us(shape) * (double)(p.dx_first ? longest(ix, a, iw, b, p.extra, groups)
+    p.us = begin_us(shape) + join_us(shape, most) + step_us(shape) * (double)(p.dx_first ? longest(ix, a, iw, b, p.extra, groups)
                                                                      : longest(iw, a, ix, b, p.extra, groups));
     return p;
 }
@@ -1019,12 +1030,13 @@ bool plan_skinny(int rows, int d, int ff) {
     return 2.5 + bytes / 8e6 < 6.0 + step_us(SINGLE) * up(d, 64) * (double)waves;
 }
 
-int plan_forward(int rows, int ff) {
+int plan_forward(int rows, int d, int ff) {
+    const int steps = up(d, 64);
     int best = SINGLE;
     double least = 0;
     for (int shape = SINGLE; shape <= TALL; ++shape) {
         const int64_t n = tiles_of(rows, ff, tile_rows(shape), tile_cols(shape) / 2), g = group_count(shape);
-        const double us = step_us(shape) * (double)((n + g - 1) / g);
+        const double us = begin_us(shape) + step_us(shape) * steps * (double)((n + g - 1) / g);
         if (shape == SINGLE || us < least) best = shape, least = us;
     }
     return best;
@@ -1035,7 +1047,7 @@ struct FfSpace { int64_t du, count, partial, bytes; };
 
 FfSpace space_of(const FfPlan& p, int rows, int ff) {
     FfSpace s;
-    s.du = (int64_t)rows * up8(ff) * 2;
+    s.du = (int64_t)rows * up64(ff) * 2;
     s.count = 2 * s.du;
     s.partial = (s.count + p.counts * 4 + 15) / 16 * 16;
     s.bytes = s.partial + p.partial_floats * 4;
@@ -1149,7 +1161,7 @@ extern "C" int scao_gated_ff_pack(const int64_t* table, int n, void* stream) {
         P.rows[i] = (int)rows;
         P.cols[i] = (int)cols;
         P.pitch[i] = t[4];
-        all += P.vecs[i] = rows * ((cols + 7) / 8);
+        all += P.vecs[i] = rows * ((cols + 63) / 64 * 8);
     }
     P.n = n;
     if ((all + 255) / 256 > 0x7fffffff) return SCAO_ERR_ARG;
@@ -1173,7 +1185,7 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     }
     FfGemm G;
     memset(&G, 0, sizeof(G));
-    const int shape = plan_forward(f->rows, f->ff), box = shape == SINGLE ? 64 : 128;
+    const int shape = plan_forward(f->rows, f->d, f->ff), box = shape == SINGLE ? 64 : 128;
     FfWork& w = G.work[0];
     w.mode = FF_FORWARD;
     w.mt = up(f->rows, tile_rows(shape));
@@ -1211,7 +1223,7 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
     FfPlan p = plan_backward(f->rows, f->d, f->ff, want_dx, want_dw);
     if (p.us < 0) return SCAO_ERR_ARG;
     const FfSpace space = space_of(p, f->rows, f->ff);
-    const int64_t ld = up8(f->ff);
+    const int64_t ld = up64(f->ff);
     char* ws = (char*)f->workspace;
     uint16_t *dg = (uint16_t*)ws, *du = (uint16_t*)(ws + space.du);
     {

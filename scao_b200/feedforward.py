@@ -48,7 +48,7 @@ def _operands(tensors):
                     continue
         if t.stride(1) != 1:
             t = t.contiguous()
-        wide = t.new_empty((t.shape[0], (n + 7) & ~7))
+        wide = t.new_empty((t.shape[0], (n + 63) & ~63))      # rows of whole 128-byte lines
         table += (t.data_ptr(), wide.data_ptr(), t.shape[0], n, t.stride(0))
         out.append((wide, wide.data_ptr(), wide.shape[1], t))
     if table:
