@@ -13,7 +13,10 @@
 //
 // Bound by HBM: one reading (plus, where c < 1, a second reading and a write;
 // the second reading runs over the tensors backwards, so it begins with what
-// the first left in L2).
+// the first left in L2).  100 M float32 values: norm 65 us (6.2 TB/s), scaling
+// 126 us (6.3 TB/s of reading and writing); 1.41 GB in 195 tensors, clipped, 684 us.
+// A single launch with a barrier between its halves would save a launch of about
+// 2 us and need every block resident.
 #include <algorithm>
 #include <new>
 #include <vector>

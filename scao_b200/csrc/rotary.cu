@@ -15,7 +15,10 @@
 //
 // A block takes a few tokens: it forms their cosines and sines once into shared
 // memory and applies them to every head of q and of k, each value read and
-// written once with the widest vector that the strides allow.  HBM bound.
+// written once with the widest vector that the strides allow.  HBM bound: 1 x 30011 x 14
+// heads x 80 float32 (64 turned, interleaved) in 48 us, 5.6 TB/s; 2 x 5000 x 40 x 128 bf16 in
+// 37 us, 5.5 TB/s.  Halves that are no whole vectors (an odd dim / 2) go value by value, at
+// 1.3 (16 bits) and 2.4 TB/s: wide own vectors with partners from L1 were no faster.
 #include <math.h>
 
 #include "common.cuh"

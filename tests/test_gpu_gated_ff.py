@@ -124,6 +124,22 @@ def test_activations(m, act, train):
     check(x, wg * 4, wu, act, train)         # gates up to about 15 both ways
 
 
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m", [2, 100])
+def test_huge_gates(m, act):
+    """Gates of 1e19 and more either way: the activation is the gate or nothing, its
+    derivative 1 or 0."""
+    x, wg, wu = (torch.ones(n, 8, dtype=torch.bfloat16, device=DEV) for n in (m, 16, 16))
+    wg[:8] *= 2.0 ** 62
+    wg[8:] *= -(2.0 ** 66)
+    ins = [v.requires_grad_() for v in (x, wg, wu)]
+    h = gated_ff(*ins, activation=act)
+    assert (h[:, :8] == 8 * 2.0 ** 62 * 8).all() and (h[:, 8:] == 0).all()
+    dx, dg, du = torch.autograd.grad(h, ins, torch.ones_like(h))
+    assert (dg[:8] == 8 * m).all() and (dg[8:] == 0).all() and (du[8:] == 0).all()
+    assert torch.isfinite(dx).all()
+
+
 @pytest.mark.parametrize("m", range(1, 70))
 def test_every_small_row_count(m):
     check(*inputs(m, 136, 72, torch.float16), "silu", False)
