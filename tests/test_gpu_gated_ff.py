@@ -518,3 +518,74 @@ def test_block_matches_its_parts():
     x = randn(2, 7, 64)
     h = gated_ff(x, block.gate.weight, block.up.weight, "gelu")
     assert torch.equal(block(x), block.out(h))
+
+
+def test_calls_from_two_threads():
+    """Forward, gradient, rotation and clipping at the same time on two streams."""
+    import threading
+
+    from scao_b200 import Rotary, clip_grad_norm_
+    sets = [inputs(m, 72, 136, torch.bfloat16, seed=m) for m in (40, 300)]
+    rotary = Rotary(24)
+
+    def work(x, wg, wu):
+        ins = [v.detach().clone().requires_grad_() for v in (x, wg, wu)]
+        h = gated_ff(*ins)
+        params = [torch.nn.Parameter(v.detach().clone()) for v in ins]
+        for p, g in zip(params, torch.autograd.grad(h, ins, torch.ones_like(h))):
+            p.grad = g
+        total = clip_grad_norm_(params, 0.5)
+        q = rotary(h.detach()[:, :120].reshape(1, -1, 5, 24).transpose(1, 2))
+        return [h.detach(), q, total, *(p.grad for p in params)]
+
+    want = [work(*s) for s in sets]
+    got, errors = [[], []], []
+    torch.cuda.synchronize()
+
+    def run(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(30):
+                    got[i].append(work(*sets[i]))
+            stream.synchronize()
+        except Exception as e:      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+def test_checkpointed_and_offloaded():
+    """Recomputed in the backward pass, or with what is kept moved to the host and back:
+    the same gradients; a graph used twice too."""
+    from torch.utils.checkpoint import checkpoint
+    block = GatedFeedForward(64, 96, device=DEV, dtype=torch.bfloat16)
+    x = randn(50, 64).requires_grad_()
+    leaves = [x, *block.parameters()]
+    dy = randn(50, 64, seed=2)
+    y = block(x)
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy)
+    other = torch.autograd.grad(checkpoint(block, x, use_reentrant=False), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = block(x)
+    moved = torch.autograd.grad(y, leaves, dy)
+    for grads in (again, other, moved):
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_backward_accumulates_into_grad():
+    ins = [v.requires_grad_() for v in inputs(20, 43, 50, torch.float16)]
+    one = torch.autograd.grad(gated_ff(*ins).sum(), ins)
+    for _ in range(2):
+        gated_ff(*ins).sum().backward()
+    for v, g in zip(ins, one):
+        assert torch.equal(v.grad, g + g)

@@ -249,3 +249,15 @@ def test_packed_arguments_match_the_structs():
     b = _lib.RotaryArgs.from_buffer_copy(rotary._ARGS.pack(*range(1, 34)))
     assert [b.src[0], b.dst[1], b.src_stride[1][0], b.dst_stride[1][2], b.turns, b.positions, b.pos_stride_b,
             b.start, b.heads[1], b.dtype, b.inverse, b.factor] == [1, 4, 8, 16, 17, 18, 19, 21, 23, 24, 31, 32]
+
+
+def test_model_copies_and_saves(tmp_path):
+    c = gpt.GPTConfig(n_layer=1, d_model=32, n_head=4, d_ff=48, vocab=50, seq_len=8, mlp="gated",
+                      positions="rotary", rotary_scaling=RotaryScaling("yarn", 4.0, original_len=8))
+    m = gpt.GPT(c)
+    torch.save(m, tmp_path / "m.pt")
+    for other in (copy.deepcopy(m), torch.load(tmp_path / "m.pt", weights_only=False)):
+        assert other.blocks[0].attn.rotary._turns == m.blocks[0].attn.rotary._turns
+        assert all(torch.equal(a, b) for a, b in zip(m.parameters(), other.parameters()))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        m(torch.arange(8)[None])
