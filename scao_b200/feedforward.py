@@ -119,7 +119,7 @@ class _GatedFF(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dh):
         need, (x, w_gate, w_up, saved) = ctx.needs_input_grad, ctx.saved_tensors
-        grads = _backward(x, w_gate, w_up, saved, dh.detach(), ctx.act, need[0], need[1] or need[2], ctx.copies)
+        grads = _backward(x, w_gate, w_up, saved, dh, ctx.act, need[0], need[1] or need[2], ctx.copies)
         if torch.is_grad_enabled():
             grads = [None if g is None else _Once.apply(g, x, w_gate, w_up, dh) for g in grads]
         return *grads, None

@@ -19,6 +19,7 @@ import struct
 from array import array
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -59,20 +60,20 @@ class RotaryScaling:
 
 
 def _frequencies(dim, base, s):
-    """(radians per position of each pair, factor on the turned values)."""
+    """(radians per position of each pair in 64 bits, factor on the turned values)."""
     if s is not None and s.kind == "ntk":
         if dim == 2:
             raise ValueError("ntk scaling needs dim > 2")
         base = base * s.factor ** (dim / (dim - 2))
-    freq = [base ** (-2.0 * j / dim) for j in range(dim // 2)]
+    freq = base ** (-np.arange(0, dim, 2, dtype=np.float64) / dim)
     if s is None or s.kind == "ntk":
         return freq, 1.0
     if s.kind == "linear":
-        return [w / s.factor for w in freq], 1.0
-    keep = [min(max((s.original_len * w / (2 * math.pi) - s.slow) / (s.fast - s.slow), 0.0), 1.0)
-            for w in freq]
+        return freq / s.factor, 1.0
+    turns = s.original_len * freq / (2 * math.pi)
+    keep = np.clip((turns - s.slow) / (s.fast - s.slow), 0.0, 1.0)
     magnitude = 0.1 * math.log(s.factor) + 1.0 if s.magnitude is None else s.magnitude
-    return [w * m + w / s.factor * (1 - m) for w, m in zip(freq, keep)], magnitude
+    return freq * keep + freq / s.factor * (1 - keep), magnitude
 
 
 class Rotary:
@@ -85,7 +86,8 @@ class Rotary:
             raise ValueError(f"rotary base must be positive, not {base}")
         self.dim, self.base, self.interleaved, self.scaling = dim, float(base), bool(interleaved), scaling
         self.frequencies, self.magnitude = _frequencies(dim, self.base, scaling)
-        self._turns = array("d", [w / (2 * math.pi) for w in self.frequencies])
+        self._turns = array("d")
+        self._turns.frombytes((self.frequencies / (2 * math.pi)).tobytes())
 
     def __call__(self, q, k=None, positions=None):
         """The turned q, or (q, k): new tensors of the same shape, type and order in
