@@ -17,8 +17,8 @@
 // memory and applies them to every head of q and of k, each value read and
 // written once with the widest vector that the strides allow.  HBM bound: 1 x 30011 x 14
 // heads x 80 float32 (64 turned, interleaved) in 48 us, 5.6 TB/s; 2 x 5000 x 40 x 128 bf16 in
-// 37 us, 5.5 TB/s.  Halves that are no whole vectors (an odd dim / 2) go value by value, at
-// 1.3 (16 bits) and 2.4 TB/s: wide own vectors with partners from L1 were no faster.
+// 37 us, 5.5 TB/s.  Where the rows allow wider vectors than their pairs do (halves of an odd
+// length, say), rotary_tile_kernel brings whole rows through shared memory.
 #include <math.h>
 
 #include "common.cuh"
@@ -40,7 +40,8 @@ struct RotArgs {
     int64_t pos_sb, pos_st, start, tokens;
     int heads[2];
     int pos64, T, D, half, tb;
-    uint32_t inv_half;                  // 2^32 / half, rounded up: i / half for i < 2^14
+    int hb;                             // heads per block (rotary_tile_kernel)
+    uint32_t inv_half, inv_per;         // of half and (rotary_tile_kernel) of a row's vectors: see small_div
     float cosm, sinm;                   // m and +-m
 };
 static_assert(sizeof(RotArgs) <= 4096, "kernel arguments");
@@ -76,6 +77,9 @@ union Pack {
     typename VecOf<sizeof(typename ElemOf<DT>::type), NV>::type v;
     typename ElemOf<DT>::type e[NV];
 };
+
+// i / n for i < 2^14, from inv = 2^32 / n rounded up (0 for n = 1)
+SCAO_DEV int small_div(int i, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)i, inv) : i; }
 
 // Item of a thread, one of S per head: NV pairs of two vectors (halves apart),
 // NV / 2 pairs of one vector (interleaved; one pair where NV is 1), or a
@@ -138,7 +142,7 @@ rotary_kernel(const __grid_constant__ RotArgs A) {
     };
     load();
     for (int i = tid; i < nt * half; i += nthr) {
-        const int t = half > 1 ? (int)__umulhi((uint32_t)i, A.inv_half) : i, j = i - t * half;
+        const int t = small_div(i, A.inv_half), j = i - t * half;
         int64_t p = base[t][4];
         if (A.pos) p = A.pos64 ? ((const int64_t*)A.pos)[p] : (int64_t)((const int32_t*)A.pos)[p];
         const int part = (int)(((uint64_t)p * A.turn[j]) >> 32);      // of a turn, times 2^32
@@ -188,6 +192,104 @@ rotary_kernel(const __grid_constant__ RotArgs A) {
     }
 }
 
+// The same over whole rows, where they allow wider vectors than their pairs do:
+// asynchronous copies of NV values each into shared memory, the pairs turned there, and the
+// rows written as wide.  With the pairs' narrow vectors too few bytes are in flight (4 x
+// 4000 x 10 x 100 bf16, 50 turned: 16 against 51 us, 92 turned: 21 against 25; float32 of
+// 96, 38 turned: 22 against 52).  Where both are as wide, rotary_kernel spares the way
+// through shared memory (2 x 5000 x 40 x 128 bf16: 37 against 52 us).
+constexpr int TILE_BYTES = 16384;       // of rows per block
+constexpr int TILE_ROWS = RT;           // at most
+
+template <int BYTES>
+SCAO_DEV void copy_async(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;"
+                 :: "r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "n"(BYTES) : "memory");
+}
+
+template <int DT, bool INTER, int NV>
+__global__ void __launch_bounds__(RT)
+rotary_tile_kernel(const __grid_constant__ RotArgs A) {
+    typedef typename ElemOf<DT>::type E;
+    typedef decltype(Pack<DT, NV>::v) Word;
+    extern __shared__ float4 tile4[];   // rows, then [token][pair] m cos, +-m sin
+    __shared__ const E* src[TILE_ROWS];
+    __shared__ E* dst[TILE_ROWS];
+    __shared__ int first[TILE_ROWS];    // of the row's cosines and sines
+    __shared__ int64_t pos[RTOK];
+    E* tile = (E*)tile4;
+    float2* cs = (float2*)((char*)tile4 + TILE_BYTES);
+    const int half = A.half, tid = threadIdx.x, H0 = A.heads[0];
+    const int64_t tok0 = (int64_t)blockIdx.x * A.tb;
+    const int nt = (int)min((int64_t)A.tb, A.tokens - tok0);
+    const int h0 = blockIdx.y * A.hb, nh = min(A.hb, H0 + A.heads[1] - h0), rows = nt * nh;
+    if (tid < rows) {
+        const int k = tid / nh, h = h0 + tid - k * nh, w = h >= H0, hh = w ? h - H0 : h;
+        const int64_t b = (tok0 + k) / A.T, t = (tok0 + k) - b * A.T;
+        src[tid] = (const E*)A.in[w] + b * A.isb[w] + t * A.ist[w] + hh * A.ish[w];
+        dst[tid] = (E*)A.out[w] + b * A.osb[w] + t * A.ost[w] + hh * A.osh[w];
+        first[tid] = k * half;
+        if (tid == k * nh) pos[k] = A.pos ? b * A.pos_sb + t * A.pos_st : A.start + t;
+    }
+    __syncthreads();
+    const int per = A.D / NV, total = rows * per;
+    for (int i = tid; i < total; i += RT) {
+        const int row = small_div(i, A.inv_per);
+        copy_async<NV * sizeof(E)>(tile + i * NV, src[row] + (i - row * per) * NV);
+    }
+    for (int i = tid; i < nt * half; i += RT) {
+        const int t = small_div(i, A.inv_half), j = i - t * half;
+        int64_t p = pos[t];
+        if (A.pos) p = A.pos64 ? ((const int64_t*)A.pos)[p] : (int64_t)((const int32_t*)A.pos)[p];
+        const int part = (int)(((uint64_t)p * A.turn[j]) >> 32);      // of a turn, times 2^32
+        float sn, c;
+        sincospif((float)part * 0x1p-31f, &sn, &c);
+        cs[i] = make_float2(A.cosm * c, A.sinm * sn);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < rows * half; i += RT) {
+        const int row = small_div(i, A.inv_half), j = i - row * half;
+        E *a = tile + row * A.D + (INTER ? 2 * j : j), *b = a + (INTER ? 1 : half);
+        const float2 q = cs[first[row] + j];
+        const float xa = to_f<DT>(*a), xb = to_f<DT>(*b);
+        *a = from_f<DT>(xa * q.x - xb * q.y);
+        *b = from_f<DT>(xa * q.y + xb * q.x);
+    }
+    __syncthreads();
+    for (int i = tid; i < total; i += RT) {
+        const int row = small_div(i, A.inv_per);
+        *(Word*)(dst[row] + (i - row * per) * NV) = *(const Word*)(tile + i * NV);
+    }
+}
+
+uint32_t inverse(int n) { return n > 1 ? (uint32_t)((0x100000000ull + n - 1) / n) : 0; }
+
+template <int DT, bool INTER, int NV>
+int launch_tile(RotArgs& A, cudaStream_t st) {
+    const int H = A.heads[0] + A.heads[1], row = A.D * (int)sizeof(typename ElemOf<DT>::type);
+    int rows = TILE_BYTES / row;                                  // at least one: see launch_width
+    if (rows > TILE_ROWS) rows = TILE_ROWS;
+    A.hb = rows < H ? rows : H;
+    int64_t tb = rows / A.hb;
+    const int64_t spread = A.tokens / (2 * scao_sm_count());
+    if (tb > spread) tb = spread;
+    if (tb > RTOK) tb = RTOK;
+    if (tb > 2048 / A.half) tb = 2048 / A.half;                   // 16 KB of cosines and sines
+    if (tb < 1) tb = 1;
+    A.tb = (int)tb;
+    A.inv_per = inverse(A.D / NV);
+    const int64_t grid = (A.tokens + tb - 1) / tb;
+    const int chunks = (H + A.hb - 1) / A.hb;
+    if (grid > 0x7fffffff || chunks > 65535) return SCAO_ERR_ARG;
+    ProfScope p(SLOT_ROTARY, st);
+    rotary_tile_kernel<DT, INTER, NV><<<dim3((unsigned)grid, chunks), RT,
+                                 TILE_BYTES + (size_t)tb * A.half * sizeof(float2), st>>>(A);
+    SCAO_CHECK_LAUNCH();
+    return SCAO_OK;
+}
+
 template <int DT, bool INTER, int NV>
 int launch(RotArgs& A, cudaStream_t st) {
     constexpr int PAIRS = INTER ? (NV > 1 ? NV / 2 : 1) : NV;
@@ -211,8 +313,14 @@ int launch(RotArgs& A, cudaStream_t st) {
     return SCAO_OK;
 }
 
+// nv: vectors of the pairs; row: of the rows
 template <int DT, bool INTER>
-int launch_width(RotArgs& A, int nv, cudaStream_t st) {
+int launch_width(RotArgs& A, int nv, int row, cudaStream_t st) {
+    if (nv < row && A.D * (int)sizeof(typename ElemOf<DT>::type) <= TILE_BYTES) {
+        if constexpr (DT != SCAO_F32)
+            if (row == 8) return launch_tile<DT, INTER, 8>(A, st);
+        return row == 4 ? launch_tile<DT, INTER, 4>(A, st) : launch_tile<DT, INTER, 2>(A, st);
+    }
     if constexpr (DT != SCAO_F32)
         if (nv == 8) return launch<DT, INTER, 8>(A, st);
     if (nv >= 4) return launch<DT, INTER, 4>(A, st);
@@ -221,8 +329,8 @@ int launch_width(RotArgs& A, int nv, cudaStream_t st) {
 }
 
 template <int DT>
-int launch_layout(RotArgs& A, bool inter, int nv, cudaStream_t st) {
-    return inter ? launch_width<DT, true>(A, nv, st) : launch_width<DT, false>(A, nv, st);
+int launch_layout(RotArgs& A, bool inter, int nv, int row, cudaStream_t st) {
+    return inter ? launch_width<DT, true>(A, nv, row, st) : launch_width<DT, false>(A, nv, row, st);
 }
 
 }  // namespace
@@ -244,14 +352,14 @@ extern "C" int scao_rotary(const ScaoRotary* r, void* stream) {
     A.cosm = r->factor;
     A.sinm = r->inverse ? -r->factor : r->factor;
     const int es = r->dtype == SCAO_F32 ? 4 : 2;
-    A.inv_half = (uint32_t)((0x100000000ull + A.half - 1) / A.half);
+    A.inv_half = inverse(A.half);
     for (int j = 0; j < A.half; ++j) {
         const double whole = floor(r->turns[j]), x = ldexp(r->turns[j] - whole, 64);
         if (!(x >= 0)) return SCAO_ERR_ARG;             // not a number, infinite
         A.turn[j] = x >= 0x1p64 ? 0 : (uint64_t)x;
     }
-    // widest vector that every address, stride and part of the head allows
-    int64_t bits = A.D | (r->interleaved ? r->dim : A.half);
+    // widest vector that every address and stride allows, and (nv) the parts of the head
+    int64_t bits = A.D;
     for (int i = 0; i < 2; ++i) {
         A.heads[i] = r->heads[i];
         if (r->heads[i] < 0) return SCAO_ERR_ARG;
@@ -270,11 +378,13 @@ extern "C" int scao_rotary(const ScaoRotary* r, void* stream) {
                 (int64_t)(((uintptr_t)A.in[i] | (uintptr_t)A.out[i]) / es);
     }
     if (A.tokens == 0 || A.heads[0] + A.heads[1] == 0) return SCAO_OK;
-    int nv = 16 / es;
-    while (nv > 1 && (bits & (nv - 1))) nv >>= 1;
+    int row = 16 / es;
+    while (row > 1 && (bits & (row - 1))) row >>= 1;
+    int nv = row;
+    while (nv > 1 && ((r->interleaved ? r->dim : A.half) & (nv - 1))) nv >>= 1;
     const cudaStream_t st = (cudaStream_t)stream;
     const bool in = r->interleaved != 0;
-    if (r->dtype == SCAO_F32) return launch_layout<SCAO_F32>(A, in, nv, st);
-    if (r->dtype == SCAO_BF16) return launch_layout<SCAO_BF16>(A, in, nv, st);
-    return launch_layout<SCAO_F16>(A, in, nv, st);
+    if (r->dtype == SCAO_F32) return launch_layout<SCAO_F32>(A, in, nv, row, st);
+    if (r->dtype == SCAO_BF16) return launch_layout<SCAO_BF16>(A, in, nv, row, st);
+    return launch_layout<SCAO_F16>(A, in, nv, row, st);
 }

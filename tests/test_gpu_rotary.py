@@ -90,6 +90,22 @@ def test_shapes(batch, heads, kv, length):
     close(r(q), q, torch.arange(length, device=DEV), r)
 
 
+@pytest.mark.parametrize("kind,head_dim,dim", [("bf16", 100, 50), ("f16", 96, 40), ("f32", 36, 14),
+                                               ("f32", 4096, 6), ("f32", 4100, 6), ("bf16", 8192, 22)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("batch,heads,kv,length", [(1, 1, 1, 1), (2, 300, 7, 3), (3, 5, 2, 700)])
+def test_rows_wider_than_their_pairs(batch, heads, kv, length, interleaved, kind, head_dim, dim):
+    """Whole rows through shared memory: heads in several blocks, rows as long as a block's
+    memory and longer."""
+    if batch * length * heads * head_dim > 1 << 26:
+        length = 5
+    r = Rotary(dim, interleaved=interleaved)
+    q, k = (randn(batch, h, length, head_dim, t=T[kind], seed=h) for h in (heads, kv))
+    ids = torch.randint(0, 1 << 20, (batch, length), device=DEV)
+    for t, y in zip((q, k), r(q, k, positions=ids)):
+        close(y, t, ids, r)
+
+
 @pytest.mark.parametrize("scaling", [None, RotaryScaling("linear", 4.0), RotaryScaling("ntk", 8.0),
                                      RotaryScaling("yarn", 16.0, original_len=4096),
                                      RotaryScaling("yarn", 2.5, original_len=100, fast=8, slow=0.5)])
