@@ -209,16 +209,18 @@ SCAO_DEV void restore4(uint32_t w0, uint32_t w1, uint32_t w2, float* v) {
 
 SCAO_DEV void ff_fail(int* status) { *(volatile int*)status = 2; }
 
-// One warp's 32 x 64 block of a result, 16-bit values in `v` (32 pairs of this
-// thread's row): through shared memory, then a TMA store or guarded stores.
-SCAO_DEV void ff_store_block(const FfWork& w, const CUtensorMap* map, int part, const uint32_t* v,
-                             unsigned char* stage, int row0, int col0, int lane) {
+// One warp's 32 x 64 block of a result, 16-bit values: into shared memory (after the
+// block before it has left), 8 columns of this thread's row at a time, then a TMA store
+// or guarded stores.
+SCAO_DEV void ff_stage_ready(int lane) {
     if (lane == 0) bulk_wait_read0();
     __syncwarp();
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-        *(uint4*)(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) =
-            make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+}
+SCAO_DEV void ff_stage_put(unsigned char* stage, int lane, int c, const uint32_t* v) {
+    *(uint4*)(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) = make_uint4(v[0], v[1], v[2], v[3]);
+}
+SCAO_DEV void ff_stage_store(const FfWork& w, const CUtensorMap* map, int part, unsigned char* stage, int row0,
+                             int col0, int lane) {
     if (w.tma_out) {
         fence_async_smem();
         __syncwarp();
@@ -273,6 +275,30 @@ SCAO_DEV void ff_store_block(const FfWork& w, const CUtensorMap* map, int part, 
         }
     }
     __syncwarp();
+}
+
+SCAO_DEV void ff_store_block(const FfWork& w, const CUtensorMap* map, int part, const uint32_t* v,
+                             unsigned char* stage, int row0, int col0, int lane) {
+    ff_stage_ready(lane);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) ff_stage_put(stage, lane, c, v + 4 * c);
+    ff_stage_store(w, map, part, stage, row0, col0, lane);
+}
+
+// 16 columns of a row from their gate and up values: kept for the gradient, and their h.
+template <int ACT>
+SCAO_DEV void ff_finish16(const FfGemm& G, const FfWork& w, const uint32_t* g, const uint32_t* u, int row, int col,
+                          uint32_t* out) {
+    if (G.saved && row < w.rows && col < w.cols) {
+        unsigned char* p = G.saved + saved_off(row, col, (w.cols + 127) >> 7);
+        save16(p, g);
+        save16(p + SAVED_BLOCK, u);
+    }
+    float y[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = ff_act<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) out[i / 2] = pack2(y[i], y[i + 1], G.dtype);
 }
 
 // The product kernel.  Roles per CTA: warp 0 TMA producer; warp 1 TMEM owner and (first
@@ -506,36 +532,42 @@ ff_gemm_kernel(const __grid_constant__ FfGemm G) {
             const int row0 = it.m * TM + 256 * half + 128 * (int)rank + q * 32, row = row0 + lane;
             const uint32_t tb = tmem + acc * TN + ((uint32_t)(q * 32) << 16);
             if constexpr (FORWARD) {
-                const int c0 = it.n * (TN / 2) + h * 64, cb = (w.cols + 127) >> 7;
-                // everything out of TMEM first, so the next item's products wait for no store
-                uint32_t gr[64], ur[64], out[32];
-#pragma unroll
-                for (int c = 0; c < 64; c += 16) {
-                    tc_ld16_async(tb + h * 64 + c, gr + c);
-                    tc_ld16_async(tb + TN / 2 + h * 64 + c, ur + c);
-                }
-#pragma unroll
-                for (int c = 0; c < 64; c += 16) {
-                    tc_ld16_wait(gr + c);
-                    tc_ld16_wait(ur + c);
-                }
-                release();
-#pragma unroll
-                for (int c = 0; c < 64; c += 16) {
-                    const uint32_t *g = gr + c, *u = ur + c;
-                    if (G.saved && row < w.rows && c0 + c < w.cols) {
-                        unsigned char* p = G.saved + saved_off(row, c0 + c, cb);
-                        save16(p, g);
-                        save16(p + SAVED_BLOCK, u);
+                const int c0 = it.n * (TN / 2) + h * 64;
+                if constexpr (!TWO) {
+                    // mostly run once: a short loop, whose instructions come from memory sooner
+                    ff_stage_ready(lane);
+#pragma unroll 1
+                    for (int c = 0; c < 64; c += 16) {
+                        uint32_t g[16], u[16], out[8];
+                        tc_ld16_async(tb + c, g);
+                        tc_ld16_async(tb + TN / 2 + c, u);
+                        tc_ld16_wait(g);
+                        tc_ld16_wait(u);
+                        ff_finish16<ACT>(G, w, g, u, row, c0 + c, out);
+                        ff_stage_put(stage, lane, c >> 3, out);
+                        ff_stage_put(stage, lane, (c >> 3) + 1, out + 4);
                     }
-                    float y[16];
+                    release();
+                    ff_stage_store(w, &G.out[0], 0, stage, row0, c0, lane);
+                } else {
+                    // everything out of TMEM first, so the next item's products wait for no store
+                    uint32_t gr[64], ur[64], out[32];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        y[i] = ff_act<ACT>(__uint_as_float(g[i])) * __uint_as_float(u[i]);
+                    for (int c = 0; c < 64; c += 16) {
+                        tc_ld16_async(tb + h * 64 + c, gr + c);
+                        tc_ld16_async(tb + TN / 2 + h * 64 + c, ur + c);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) out[(c + i) / 2] = pack2(y[i], y[i + 1], G.dtype);
+                    for (int c = 0; c < 64; c += 16) {
+                        tc_ld16_wait(gr + c);
+                        tc_ld16_wait(ur + c);
+                    }
+                    release();
+#pragma unroll
+                    for (int c = 0; c < 64; c += 16)
+                        ff_finish16<ACT>(G, w, gr + c, ur + c, row, c0 + c, out + c / 2);
+                    ff_store_block(w, &G.out[0], 0, out, stage, row0, c0, lane);
                 }
-                ff_store_block(w, &G.out[0], 0, out, stage, row0, c0, lane);
             } else {
                 constexpr int COLS = TN / 2;            // of this warp
                 const int cw = h * COLS;
@@ -911,21 +943,24 @@ int tile_rows(int shape) { return shape == SINGLE ? 128 : shape == PAIR ? 256 : 
 int tile_cols(int shape) { return shape == SINGLE ? 128 : 256; }
 int group_count(int shape) { return scao_sm_count() / (shape == SINGLE ? 1 : 2); }
 
-// Steps that the busiest group runs, as ff_item deals the items out: na of la steps, then
-// nb of lb.
-int64_t longest(int64_t na, int64_t la, int64_t nb, int64_t lb, int extra, int G) {
+// Time of the busiest group, as ff_item deals the items out: na of ta each, then nb of tb.
+double longest(int64_t na, double ta, int64_t nb, double tb, int extra, int G) {
     const int64_t h = na / G, r = na % G, early = r ? (G - r) * extra < nb ? (G - r) * extra : nb : 0;
-    const int64_t rest = (nb - early + G - 1) / G * lb;
-    const int64_t x = (h + (r > 0)) * la + rest, y = h * la + (early ? extra : 0) * lb + rest;
+    const double rest = (double)((nb - early + G - 1) / G) * tb;
+    const double x = (double)(h + (r > 0)) * ta + rest, y = (double)h * ta + (early ? extra : 0) * tb + rest;
     return x > y ? x : y;
 }
 
 // Microseconds, measured, of which the plan is chosen.  A step of a tile: a CTA takes in
 // about 50 bytes of operands a clock, whatever the shape, so the 32 KB of SINGLE and PAIR
 // bound their steps (the tensor cores need 256 and 512 clocks of them), the 48 KB of TALL
-// take about its 1024 clocks.  Set-up, first copies and the last epilogue, beyond SINGLE's.
-// Joining a tile's shares.
+// take about its 1024 clocks.  An epilogue, which an item of few steps waits for.  Set-up,
+// first copies and the last epilogue, beyond SINGLE's.  Joining a tile's shares.
 double step_us(int shape) { return shape == SINGLE ? 0.35 : shape == PAIR ? 0.40 : 0.72; }
+double item_us(int shape, int steps) {
+    const double epilogue = shape == SINGLE ? 1.6 : shape == PAIR ? 2.4 : 4.8, main = step_us(shape) * steps;
+    return main > epilogue ? main : epilogue;
+}
 double begin_us(int shape) { return shape == SINGLE ? 0.0 : shape == PAIR ? 1.2 : 1.6; }
 double join_us(int shape, int splits) {
     return splits == 1 ? 0.0 : shape == SINGLE ? 1.5 + 0.3 * splits : 4.0 + 1.0 * splits;
@@ -981,30 +1016,33 @@ FfPlan plan_shape(int shape, int rows, int d, int ff, int dx_splits, int dw_spli
     p.dx_items = (int)ix;
     p.dw_items = (int)iw;
     // the product with the longer items first
-    const int lx = nx ? up(p.dx.steps, p.dx.splits) : 0, lw = nw ? up(p.dw.steps, p.dw.splits) : 0;
-    p.dx_first = lx >= lw;
-    const int a = p.dx_first ? lx : lw, b = p.dx_first ? lw : lx;
-    p.extra = b ? (a + b / 2) / b : 0;
+    const double tx = nx ? item_us(shape, up(p.dx.steps, p.dx.splits)) : 0;
+    const double tw = nw ? item_us(shape, up(p.dw.steps, p.dw.splits)) : 0;
+    p.dx_first = tx >= tw;
+    const double a = p.dx_first ? tx : tw, b = p.dx_first ? tw : tx;
+    p.extra = b > 0 ? (int)(a / b + 0.5) : 0;
     const int most = p.dx.splits > p.dw.splits ? p.dx.splits : p.dw.splits;
-    p.us = begin_us(shape) + join_us(shape, most) + step_us(shape) * (double)(p.dx_first ? longest(ix, a, iw, b, p.extra, groups)
-                                                                     : longest(iw, a, ix, b, p.extra, groups));
+    p.us = begin_us(shape) + join_us(shape, most) +
+           (p.dx_first ? longest(ix, a, iw, b, p.extra, groups) : longest(iw, a, ix, b, p.extra, groups));
     return p;
 }
 
-// The shape and the number of items whose busiest group is done first.  Where the tiles
-// leave groups idle, items of 8 steps and more are tried, in lengths a fifth apart.
+// The shape and the cut whose busiest group is done first.  Cuts: items of 8 steps and
+// more, in lengths a fifth apart, of the products that are longer than that, while their
+// shares are no more than the groups.
 FfPlan plan_backward_new(int rows, int d, int ff, bool want_dx, bool want_dw) {
     FfPlan best = plan_shape(TALL, rows, d, ff, want_dx, want_dw);
     auto take = [&](const FfPlan& p) { if (best.us < 0 || (p.us >= 0 && p.us < best.us)) best = p; };
     for (int shape = SINGLE; shape <= PAIR; ++shape) {
         const FfPlan whole = plan_shape(shape, rows, d, ff, want_dx, want_dw);
         take(whole);
+        if (whole.us < 0) continue;
         const int64_t nx = whole.dx_items, nw = whole.dw_items, groups = group_count(shape);
-        if (whole.us < 0 || nx + nw >= groups) continue;
         const int most = whole.dx.steps > whole.dw.steps ? whole.dx.steps : whole.dw.steps;
         for (int64_t len = 8; len < most; len += len / 5 > 1 ? len / 5 : 1) {
             const int sx = want_dx ? up(whole.dx.steps, (int)len) : 0, sw = want_dw ? up(whole.dw.steps, (int)len) : 0;
-            if (nx * sx + nw * sw <= groups) take(plan_shape(shape, rows, d, ff, sx, sw));
+            if ((sx > 1 ? nx * sx : 0) + (sw > 1 ? nw * sw : 0) <= groups)
+                take(plan_shape(shape, rows, d, ff, sx, sw));
         }
     }
     return best;
