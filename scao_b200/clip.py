@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import math
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -19,6 +20,8 @@ from . import _lib
 from .cuda import _CODE, _launch
 
 _KIND = {1.0: 0, 2.0: 1, math.inf: 2}
+_DTYPES = set(_CODE)
+_DTYPE, _LAYOUT, _GRAD = attrgetter("dtype"), attrgetter("layout"), attrgetter("grad")
 
 
 def _layout(t):
@@ -51,11 +54,11 @@ def _table(tensors, write):
     device number).  Strided gradients that are not dense are packed for the call; tensors
     that will be written must not share memory."""
     n, index = len(tensors), tensors[0].get_device()
-    codes = [_CODE.get(t.dtype, -1) for t in tensors]
-    get = torch.Tensor
-    if index < 0 or -1 in codes or list(map(get.get_device, tensors)).count(index) != n or \
-            [t.layout for t in tensors].count(torch.strided) != n:
+    get, dtypes = torch.Tensor, set(map(_DTYPE, tensors))
+    if index < 0 or not dtypes <= _DTYPES or set(map(get.get_device, tensors)) != {index} or \
+            set(map(_LAYOUT, tensors)) != {torch.strided}:
         _refuse(tensors)
+    codes = [_CODE[dtypes.pop()]] * n if len(dtypes) == 1 else [_CODE[t.dtype] for t in tensors]
     packed = []
     if not all(map(get.is_contiguous, tensors)):
         tensors = list(tensors)
@@ -101,7 +104,7 @@ def _max_norm(max_norm):
 def _grads(parameters):
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    return [g for g in [p.grad for p in parameters] if g is not None]
+    return [g for g in map(_GRAD, parameters) if g is not None]
 
 
 def _refuse_nonfinite(total, norm_type):
