@@ -15,6 +15,7 @@ CUDA tensors of one device.
 from __future__ import annotations
 
 import math
+import operator
 import struct
 from array import array
 from dataclasses import dataclass
@@ -110,7 +111,7 @@ class Rotary:
                     (positions.dim() == 2 and positions.shape[0] not in (1, q.shape[0])):
                 raise ValueError(f"positions {tuple(positions.shape)} do not fit q {tuple(q.shape)}")
         elif positions is not None:
-            start, positions = int(positions), None
+            start, positions = operator.index(positions), None
             if abs(start) >= 1 << 52:
                 raise ValueError(f"position {start} is out of range")
         index = q.get_device()
@@ -118,7 +119,7 @@ class Rotary:
                 (positions is not None and positions.get_device() != index):
             raise RuntimeError("scao_b200: q, k and positions must be on one CUDA device (no CPU path)")
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-            out = _Turn.apply(self, False, positions, start, index, q, k)
+            out = _Turn.apply((self, False, start, index), positions, q, k)
         else:
             out = _run(self, False, positions, start, index, (q, k))
         return out[0] if k is None else tuple(out)
@@ -174,20 +175,23 @@ class _Turn(torch.autograd.Function):
     """The rotation, or its transpose (``inverse``), which is its gradient."""
 
     @staticmethod
-    def forward(ctx, rotary, inverse, positions, start, index, q, k):
-        ctx.args = rotary, inverse, start, index
-        ctx.save_for_backward(positions)
+    def forward(ctx, how, positions, q, k):
+        ctx.how = how
+        if positions is not None:
+            ctx.save_for_backward(positions)
         ctx.set_materialize_grads(False)
+        rotary, inverse, start, index = how
         return tuple(_run(rotary, inverse, positions, start, index, (q, k)))
 
     @staticmethod
     def backward(ctx, gq, gk):
-        rotary, inverse, start, index = ctx.args
-        (positions,) = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        gq, gk = gq if need[5] else None, gk if need[6] else None
+        rotary, inverse, start, index = ctx.how
+        saved = ctx.saved_tensors
+        positions = saved[0] if saved else None
+        _, _, need_q, need_k = ctx.needs_input_grad
+        gq, gk = gq if need_q else None, gk if need_k else None
         if torch.is_grad_enabled():                         # differentiable again
-            gq, gk = _Turn.apply(rotary, not inverse, positions, start, index, gq, gk)
+            gq, gk = _Turn.apply((rotary, not inverse, start, index), positions, gq, gk)
         else:
             gq, gk = _run(rotary, not inverse, positions, start, index, (gq, gk))
-        return None, None, None, None, None, gq, gk
+        return None, None, gq, gk

@@ -122,6 +122,8 @@ def test_rotary_refuses_tensors():
             r(q, positions=p)
     with pytest.raises(TypeError, match="int32 or int64"):
         r(q, positions=torch.zeros(5))
+    with pytest.raises(TypeError):
+        r(q, positions=2.5)
     with pytest.raises(RuntimeError, match="CUDA"):
         r(q)
 
