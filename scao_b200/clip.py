@@ -15,9 +15,10 @@ from array import array
 from operator import attrgetter
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .cuda import _CODE, _launch
+from .cuda import _CODE, _followed, _launch
 
 _KIND = {1.0: 0, 2.0: 1, math.inf: 2}
 _DTYPES = set(_CODE)
@@ -54,6 +55,8 @@ def _table(tensors, write):
     device number).  Strided gradients that are not dense are packed for the call; tensors
     that will be written must not share memory."""
     n, index = len(tensors), tensors[0].get_device()
+    if _followed() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("gradients with forward-mode tangents are not clipped")
     get, dtypes = torch.Tensor, set(map(_DTYPE, tensors))
     if index < 0 or not dtypes <= _DTYPES or set(map(get.get_device, tensors)) != {index} or \
             set(map(_LAYOUT, tensors)) != {torch.strided}:

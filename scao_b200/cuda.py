@@ -10,6 +10,7 @@ RuntimeError, as does any error status of the library call.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -26,6 +27,12 @@ def _on_cuda(*ts):
 
 def _stream(dev):
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _followed():
+    """Whether forward-mode derivatives may follow the call: they see an autograd function
+    (and raise, where it has none for them), but not a launch into a new tensor."""
+    return forward_ad._current_level >= 0
 
 
 def _launch(what, index, fn, *args):

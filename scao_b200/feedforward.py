@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .cuda import _CODE, _launch
+from .cuda import _CODE, _followed, _launch
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
@@ -120,14 +120,14 @@ class _GatedFF(torch.autograd.Function):
     def backward(ctx, dh):
         need, (x, w_gate, w_up, saved) = ctx.needs_input_grad, ctx.saved_tensors
         grads = _backward(x, w_gate, w_up, saved, dh, ctx.act, need[0], need[1] or need[2], ctx.copies)
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or _followed():
             grads = [None if g is None else _Once.apply(g, x, w_gate, w_up, dh) for g in grads]
         return *grads, None
 
 
 def gated_ff(x, w_gate, w_up, activation="silu"):
     """act(x w_gate^T) * (x w_up^T): module docstring.  Differentiable once in x and the
-    weights."""
+    weights; forward-mode derivatives raise."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, not {activation!r}")
@@ -148,7 +148,7 @@ def gated_ff(x, w_gate, w_up, activation="silu"):
     if not x.is_cuda or w_gate.get_device() != x.get_device() or w_up.get_device() != x.get_device():
         raise RuntimeError("scao_b200: x, w_gate and w_up must be on one CUDA device (no CPU path)")
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+    if _followed() or torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
         h = _GatedFF.apply(flat, w_gate, w_up, act)
     else:
         h = _forward(flat, w_gate, w_up, act, False)[0]

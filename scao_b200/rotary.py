@@ -7,7 +7,7 @@
 
 Pair j of a head at position p turns by p w_j, w_j = base^(-2j / dim); the pair is
 (2j, 2j + 1) where ``interleaved``, else (j, j + dim / 2); values from ``dim`` on pass
-through.  Angles are formed in 64 bits, so far positions stay exact.  Any strides with
+through.  Forward-mode derivatives raise.  Angles are formed in 64 bits, so far positions stay exact.  Any strides with
 neighbouring values of a head next to each other are read as they are (views of a fused
 projection, (batch, length, heads, head_dim) memory).  float32, bfloat16 and float16,
 CUDA tensors of one device.
@@ -24,7 +24,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .cuda import _CODE, _launch
+from .cuda import _CODE, _followed, _launch
 
 MAX_DIM = 512
 
@@ -118,7 +118,7 @@ class Rotary:
         if not q.is_cuda or (k is not None and k.get_device() != index) or \
                 (positions is not None and positions.get_device() != index):
             raise RuntimeError("scao_b200: q, k and positions must be on one CUDA device (no CPU path)")
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if _followed() or torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             out = _Turn.apply((self, False, start, index), positions, q, k)
         else:
             out = _run(self, False, positions, start, index, (q, k))
@@ -190,7 +190,7 @@ class _Turn(torch.autograd.Function):
         positions = saved[0] if saved else None
         _, _, need_q, need_k = ctx.needs_input_grad
         gq, gk = gq if need_q else None, gk if need_k else None
-        if torch.is_grad_enabled():                         # differentiable again
+        if torch.is_grad_enabled() or _followed():          # differentiable again
             gq, gk = _Turn.apply((rotary, not inverse, start, index), positions, gq, gk)
         else:
             gq, gk = _run(rotary, not inverse, positions, start, index, (gq, gk))

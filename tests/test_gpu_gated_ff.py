@@ -589,3 +589,24 @@ def test_backward_accumulates_into_grad():
         gated_ff(*ins).sum().backward()
     for v, g in zip(ins, one):
         assert torch.equal(v.grad, g + g)
+
+
+def test_forward_mode_is_refused():
+    """A tangent is refused, as an input's and as a gradient's; a level without one changes nothing."""
+    from torch.autograd import forward_ad
+    x, wg, wu = inputs(40, 64, 48, torch.bfloat16)
+    leaf, dh = x.clone().requires_grad_(), randn(40, 48, seed=5)
+    want = gated_ff(leaf, wg, wu)
+    (dx,) = torch.autograd.grad(want, leaf, dh, retain_graph=True)
+    with forward_ad.dual_level():
+        for i in range(3):
+            ins = [forward_ad.make_dual(v, v) if k == i else v for k, v in enumerate((x, wg, wu))]
+            with pytest.raises(NotImplementedError), torch.no_grad():
+                gated_ff(*ins)
+            with pytest.raises(NotImplementedError):
+                gated_ff(*ins)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(want, leaf, forward_ad.make_dual(dh, dh), retain_graph=True)
+        h = gated_ff(leaf, wg, wu)
+        assert torch.equal(h, want) and torch.equal(gated_ff(x, wg, wu), want)
+        assert torch.equal(torch.autograd.grad(h, leaf, dh)[0], dx)

@@ -232,3 +232,21 @@ def test_long_batch_offsets_pass_32_bits():
     y = torch.empty(1, 2, 3, 64, dtype=torch.bfloat16, device=DEV)
     y = r(x)
     close(y, x, torch.arange(3, device=DEV), r)
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+    r, q, k = Rotary(16), randn(1, 2, 5, 16), randn(1, 1, 5, 16, seed=1)
+    leaf = q.clone().requires_grad_()
+    want = r(leaf)
+    (dq,) = torch.autograd.grad(want, leaf, q, retain_graph=True)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, q)
+        for args in ((dual,), (dual, k), (k, dual)):
+            with pytest.raises(NotImplementedError):
+                r(*args)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(want, leaf, dual, retain_graph=True)
+        y = r(leaf)
+        assert torch.equal(y, want) and torch.equal(r(q), want)
+        assert torch.equal(torch.autograd.grad(y, leaf, q)[0], dq)

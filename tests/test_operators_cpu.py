@@ -58,6 +58,18 @@ def test_clip_refuses_shared_memory():
         clip_grad_norm_([param(base[:10]), param(base[10:])], 1.0)
 
 
+def test_clip_refuses_forward_mode():
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(torch.ones(3), torch.ones(3))
+        with pytest.raises(NotImplementedError, match="tangents"):
+            clip_grad_norm_([param(torch.ones(2)), param(g)], 1.0)
+        with pytest.raises(NotImplementedError, match="tangents"):
+            get_total_norm([g])
+        with pytest.raises(RuntimeError, match="CUDA"):
+            get_total_norm([torch.ones(3)])
+
+
 def test_clip_without_gradients():
     assert clip_grad_norm_([torch.nn.Parameter(torch.ones(2))], 1.0).item() == 0
     assert clip_grads_with_norm_([], 1.0, torch.ones(())) is None
