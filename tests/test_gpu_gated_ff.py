@@ -610,3 +610,20 @@ def test_forward_mode_is_refused():
         h = gated_ff(leaf, wg, wu)
         assert torch.equal(h, want) and torch.equal(gated_ff(x, wg, wu), want)
         assert torch.equal(torch.autograd.grad(h, leaf, dh)[0], dx)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("d", [64, 63])
+@pytest.mark.parametrize("grad", [False, True])
+def test_traces(grad, d):
+    """A torch.jit trace calls the operator again, in both directions; an FX trace is refused."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, wg, wu = inputs(40, d, 48, torch.bfloat16)
+    call = lambda v: gated_ff(v, wg, wu)  # noqa: E731
+    traced = torch.jit.trace(call, x.clone().requires_grad_(grad), check_trace=False)
+    other = randn(40, d, seed=9).requires_grad_()
+    h, want = traced(other), call(other)
+    assert torch.equal(h, want)
+    assert torch.equal(torch.autograd.grad(h.sum(), other)[0], torch.autograd.grad(want.sum(), other)[0])
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(call)(x.clone().requires_grad_(grad))

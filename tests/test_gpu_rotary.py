@@ -250,3 +250,19 @@ def test_forward_mode_is_refused():
         y = r(leaf)
         assert torch.equal(y, want) and torch.equal(r(q), want)
         assert torch.equal(torch.autograd.grad(y, leaf, q)[0], dq)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("grad", [False, True])
+def test_traces(grad):
+    """A torch.jit trace calls the operator again, in both directions; an FX trace is refused."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    r, ids = Rotary(16), torch.arange(5, device=DEV) + 9
+    for call in (lambda t: r(t), lambda t: r(t, t[:, :1], positions=ids)[1], lambda t: r(t, t, positions=3)[0]):
+        traced = torch.jit.trace(call, randn(1, 2, 5, 16).requires_grad_(grad), check_trace=False)
+        other = randn(1, 2, 5, 16, seed=9).requires_grad_()
+        y, want = traced(other), call(other)
+        assert torch.equal(y, want)
+        assert torch.equal(torch.autograd.grad(y.sum(), other)[0], torch.autograd.grad(want.sum(), other)[0])
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(call)(randn(1, 2, 5, 16).requires_grad_(grad))

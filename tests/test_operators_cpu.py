@@ -101,6 +101,21 @@ def test_clip_c_entry_checks():
     assert L.scao_grad_norm_workspace_bytes(1) <= L.scao_grad_norm_workspace_bytes(5000)
 
 
+@pytest.mark.parametrize("pre_dispatch", [False, True])
+def test_fx_traces_are_refused(pre_dispatch):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from scao_b200.cuda import _launch
+
+    def call(x):
+        y = x.new_empty(3)
+        _launch("scao_rotary", 0, lambda *args: 0)
+        return y
+
+    with pytest.raises(RuntimeError, match="scao_rotary cannot be traced"):
+        make_fx(call, pre_dispatch=pre_dispatch)(torch.ones(3))
+
+
 # -------------------------------------------------------------------- rotary
 @pytest.mark.parametrize("dim", [0, 1, 3, -2, 514])
 def test_rotary_refuses_dims(dim):
