@@ -627,3 +627,22 @@ def test_traces(grad, d):
     assert torch.equal(torch.autograd.grad(h.sum(), other)[0], torch.autograd.grad(want.sum(), other)[0])
     with pytest.raises(RuntimeError, match="cannot be traced"):
         make_fx(call)(x.clone().requires_grad_(grad))
+
+
+def test_first_calls_from_threads():
+    """The first calls of a process may come from several threads at once."""
+    import subprocess
+    import sys
+    code = ("import sys, threading, torch; from scao_b200 import _lib, gated_ff\n"
+            "_lib.lib(); sys.setswitchinterval(1e-6)\n"
+            "x = torch.randn(100, 64, device='cuda').bfloat16(); w = torch.randn(48, 64, device='cuda').bfloat16()\n"
+            "torch.cuda.synchronize(); gate = threading.Barrier(16); out = [None] * 16\n"
+            "def run(i):\n"
+            "    torch.cuda.set_device(0); gate.wait()\n"
+            "    out[i] = gated_ff(x, w, w)\n"
+            "threads = [threading.Thread(target=run, args=(i,)) for i in range(16)]\n"
+            "[t.start() for t in threads]; [t.join() for t in threads]\n"
+            "assert all(torch.equal(h, gated_ff(x, w, w)) for h in out)\n")
+    for _ in range(3):
+        r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stderr[-2000:]
