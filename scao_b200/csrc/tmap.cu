@@ -28,6 +28,15 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
+// Runs an encode.  The driver wants the device's context current in the calling thread; the
+// runtime makes it so at a thread's first work, which this may be: then set it and try again.
+template <class Encode>
+bool with_context(const Encode& encode) {
+    if (encode()) return true;
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode();
+}
+
 }  // namespace
 
 bool scao_build_tensor_maps(const ScaoPlanDev* P, const ScaoParam* ph, const ScaoParamStep* sh,
@@ -43,9 +52,11 @@ bool scao_build_tensor_maps(const ScaoPlanDev* P, const ScaoParam* ph, const Sca
         const cuuint64_t strides[1] = {(cuuint64_t)cols * es};
         const cuuint32_t box[2] = {bx, by};
         const cuuint32_t estr[2] = {1, 1};
-        return enc(m, t, 2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
-               CUDA_SUCCESS;
+        return with_context([&] {
+            return enc(m, t, 2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+                   CUDA_SUCCESS;
+        });
     };
     const auto BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, F4 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     const auto SW = CU_TENSOR_MAP_SWIZZLE_128B, NS = CU_TENSOR_MAP_SWIZZLE_NONE;
@@ -83,11 +94,13 @@ bool scao_tensor_map_2d(void* map, int dtype, const void* base, int64_t rows, in
     const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
     const cuuint32_t box[2] = {(cuuint32_t)bx, (cuuint32_t)by};
     const cuuint32_t estr[2] = {1, 1};
-    return enc((CUtensorMap*)map,
-               dtype == SCAO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-               (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return with_context([&] {
+        return enc((CUtensorMap*)map,
+                   dtype == SCAO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                   (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    });
 }
 
 int scao_sm_count() {

@@ -646,3 +646,30 @@ def test_first_calls_from_threads():
     for _ in range(3):
         r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
         assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_first_work_of_a_thread():
+    """A call may be the first GPU work of its thread."""
+    import threading
+    x, wg, wu = inputs(100, 64, 48, torch.bfloat16)
+    want = gated_ff(x, wg, wu)
+    leaf = x.clone().requires_grad_()
+    kept = gated_ff(leaf, wg, wu)
+    (dx,) = torch.autograd.grad(kept, leaf, want, retain_graph=True)
+    torch.cuda.synchronize()
+    got = {}
+
+    def run(name, call):
+        try:
+            got[name] = call()
+        except Exception as e:      # noqa: BLE001
+            got[name] = e
+
+    for name, call in (("forward", lambda: gated_ff(x, wg, wu)),
+                       ("gradient", lambda: torch.autograd.grad(kept, leaf, want)[0])):
+        t = threading.Thread(target=run, args=(name, call))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert not any(isinstance(v, Exception) for v in got.values()), got
+    assert torch.equal(got["forward"], want) and torch.equal(got["gradient"], dx)
