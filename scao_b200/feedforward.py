@@ -32,25 +32,26 @@ _ARGS = struct.Struct("@10P4q6i")
 def _operands(tensors):
     """The 2-D ``tensors`` as the kernels read them (neighbouring values of a row adjacent,
     rows a multiple of 16 bytes apart, the first on 16 bytes; copies, in one launch,
-    where they lie otherwise): ([tensor, address, row pitch] of each, whether any was
-    copied)."""
-    out, table = [], []
+    where they lie otherwise): ([tensor, address, row pitch, whether a copy] of each,
+    whether any was copied)."""
+    out, table, kept = [], [], []
     for t in tensors:
         n, p = t.shape[1], t.data_ptr()
         if p & 15 == 0:
             if n & 7 == 0 and t.is_contiguous():
-                out.append((t, p, n))
+                out.append((t, p, n, False))
                 continue
             if t.stride(1) == 1 or n == 1:
                 pitch = t.stride(0) if t.shape[0] > 1 else (n + 7) & ~7
                 if pitch & 7 == 0 and pitch >= n:
-                    out.append((t, p, pitch))
+                    out.append((t, p, pitch, False))
                     continue
         if t.stride(1) != 1:
             t = t.contiguous()
+            kept.append(t)
         wide = t.new_empty((t.shape[0], (n + 63) & ~63))      # rows of whole 128-byte lines
         table += (t.data_ptr(), wide.data_ptr(), t.shape[0], n, t.stride(0))
-        out.append((wide, wide.data_ptr(), wide.shape[1], t))
+        out.append((wide, wide.data_ptr(), wide.shape[1], True))
     if table:
         table = array("q", table)
         _launch("scao_gated_ff_pack", tensors[0].get_device(), _lib.lib().scao_gated_ff_pack,
@@ -59,31 +60,30 @@ def _operands(tensors):
 
 
 def _forward(x, w_gate, w_up, act, train):
-    """(h, what the gradient reads or None, copies of operands or None)."""
+    """(h, what the gradient reads or None, [the copy of each operand or None])."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
     h = x.new_empty((rows, ff))
-    saved = copies = None
+    saved, copies = None, (None, None, None)
     if train:
         saved = x.new_empty(L.scao_gated_ff_saved_bytes(rows, ff) >> 1)     # 16-bit places
     if rows:
-        ins, copied = _operands((x, w_gate, w_up))
+        ins, _ = _operands((x, w_gate, w_up))
         args = _ARGS.pack(ins[0][1], ins[1][1], ins[2][1], h.data_ptr(), saved.data_ptr() if train else 0,
                           0, 0, 0, 0, 0, ins[0][2], ins[1][2], ins[2][2], 0,
                           rows, d, ff, _CODE[x.dtype], act, 0)
         _launch("scao_gated_ff_forward", x.get_device(), L.scao_gated_ff_forward, args)
-        if copied and train:
-            copies = [i[0] for i in ins]
+        copies = [i[0] if i[3] else None for i in ins]
     return h, saved, copies
 
 
-def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w, copies=None):
+def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w, copies):
     """(dx, dw_gate, dw_up), None where not needed."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
     dx = x.new_empty((rows, d)) if need_x else None
     new = x.new_empty if rows else x.new_zeros
     dwg, dwu = (new((ff, d)), new((ff, d))) if need_w else (None, None)
     if rows:
-        ins, _ = _operands(copies or (x, w_gate, w_up))
+        ins, _ = _operands([t if c is None else c for t, c in zip((x, w_gate, w_up), copies)])
         if dh.stride(1) != 1:
             dh = dh.contiguous()
         ws = x.new_empty((L.scao_gated_ff_workspace_bytes(rows, d, ff, need_x | need_w << 1) + 1) >> 1)
@@ -111,15 +111,15 @@ class _Once(torch.autograd.Function):
 class _GatedFF(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act):
-        h, saved, ctx.copies = _forward(x, w_gate, w_up, act, True)
+        h, saved, copies = _forward(x, w_gate, w_up, act, True)
         ctx.act = act
-        ctx.save_for_backward(x, w_gate, w_up, saved)
+        ctx.save_for_backward(x, w_gate, w_up, saved, *copies)
         return h
 
     @staticmethod
     def backward(ctx, dh):
-        need, (x, w_gate, w_up, saved) = ctx.needs_input_grad, ctx.saved_tensors
-        grads = _backward(x, w_gate, w_up, saved, dh, ctx.act, need[0], need[1] or need[2], ctx.copies)
+        need, (x, w_gate, w_up, saved, *copies) = ctx.needs_input_grad, ctx.saved_tensors
+        grads = _backward(x, w_gate, w_up, saved, dh, ctx.act, need[0], need[1] or need[2], copies)
         if torch.is_grad_enabled() or _followed():
             grads = [None if g is None else _Once.apply(g, x, w_gate, w_up, dh) for g in grads]
         return *grads, None

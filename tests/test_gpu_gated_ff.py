@@ -673,3 +673,48 @@ def test_first_work_of_a_thread():
     torch.cuda.synchronize()
     assert not any(isinstance(v, Exception) for v in got.values()), got
     assert torch.equal(got["forward"], want) and torch.equal(got["gradient"], dx)
+
+
+def test_copies_for_the_gradient_are_saved_tensors():
+    """Aligned copies go where saved tensors go: to the host and back, recomputed, and freed
+    with them; operands that lie right are not kept twice."""
+    from torch.utils.checkpoint import checkpoint
+    m, d, f = 300, 1021, 520
+    ins = [v.requires_grad_() for v in inputs(m, d, f, torch.float16)]
+    dh = randn(m, f, t=torch.float16, seed=5)
+    saved = (m + 127) // 128 * ((f + 127) // 128) * 128 * 128 * 6
+    copies = (m + 2 * f) * 1024 * 2
+    used = lambda: torch.cuda.memory_stats()["requested_bytes.all.current"]  # noqa: E731
+
+    def kept(context):
+        """(memory held between the passes, after the backward pass, the gradients)"""
+        torch.cuda.synchronize()
+        start = used()
+        with context:
+            h = gated_ff(*ins)
+        held = used() - start - h.numel() * 2
+        loss = (h * dh).sum()       # holds the graph
+        del h
+        grads = torch.autograd.grad(loss, ins)
+        after = used() - start - sum(g.numel() * 2 for g in grads)
+        return held, after, grads, loss
+
+    import contextlib
+    held, after, want, loss = kept(contextlib.nullcontext())
+    assert saved + copies <= held < saved + copies + 8192
+    assert after < 8192, after
+    held, _, grads, loss = kept(torch.autograd.graph.save_on_cpu())
+    assert held < 8192, held
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+    torch.cuda.synchronize()
+    start = used()
+    h = checkpoint(gated_ff, *ins, use_reentrant=False)
+    assert used() - start - h.numel() * 2 < 8192
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad((h * dh).sum(), ins), want))
+    x = ins[0].detach()
+    wide = torch.empty(m, 1024, dtype=x.dtype, device=DEV)[:, :d].copy_(x).requires_grad_()     # only the weights lie odd
+    torch.cuda.synchronize()
+    start = used()
+    h = gated_ff(wide, *ins[1:])
+    assert used() - start - h.numel() * 2 < saved + 2 * f * 1024 * 2 + 8192
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(h, [wide, *ins[1:]], dh), want))
