@@ -247,7 +247,7 @@ SCAO_DEV void ff_stage_store(const FfWork& w, const CUtensorMap* map, int part, 
             if (r < rows && 2 * lane < cols)
                 *(uint32_t*)(out + (row0 + r) * w.ldo + 2 * lane) = *(const uint32_t*)at(r, 2 * lane);
     } else {
-        // an odd pitch: every other row begins between two 32-bit words, and a lane's
+        // a row that begins between two 32-bit words (every other one of an odd pitch): a lane's
         // word is then the upper half of its pair and the lower half of the next lane's
         uint16_t* d = out + row0 * w.ldo;
         auto even = [&](int r) {
@@ -266,7 +266,11 @@ SCAO_DEV void ff_stage_store(const FfWork& w, const CUtensorMap* map, int part, 
             else if (2 * lane + 1 < cols) *p = (uint16_t)(x >> 16);
             if (lane == 0 && cols > 0) p[-1] = (uint16_t)x;
         };
-        if ((uintptr_t)d & 2) {
+        if (!(w.ldo & 1)) {                 // a result that begins so: all its rows alike
+#pragma unroll 1
+            for (int r = 0; r < 32; ++r)
+                if ((uintptr_t)d & 2) odd(r); else even(r);
+        } else if ((uintptr_t)d & 2) {
 #pragma unroll 4
             for (int r = 0; r < 32; r += 2) { odd(r); even(r + 1); }
         } else {

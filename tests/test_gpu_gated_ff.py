@@ -718,3 +718,34 @@ def test_copies_for_the_gradient_are_saved_tensors():
     h = gated_ff(wide, *ins[1:])
     assert used() - start - h.numel() * 2 < saved + 2 * f * 1024 * 2 + 8192
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(h, [wide, *ins[1:]], dh), want))
+
+
+@pytest.mark.parametrize("f", [40, 41, 42])
+@pytest.mark.parametrize("m,d", [(40, 64), (130, 63), (300, 66)])
+@pytest.mark.parametrize("at", [(1, 1, 1, 1), (2, 2, 2, 1), (3, 5, 1, 4), (4, 6, 7, 7)])
+def test_results_anywhere(at, m, d, f):
+    """Through the C entry: results that begin between two 32-bit words, of even and odd
+    pitch, each of its own alignment; the same bits, and nothing beside them."""
+    import ctypes
+    x, wg, wu = (torch.nn.functional.pad(v, (0, -d % 8)) for v in inputs(m, d, f, torch.bfloat16))
+    L, stream, ld = _lib.lib(), torch.cuda.current_stream().cuda_stream, x.shape[1]
+    saved = torch.empty(int(L.scao_gated_ff_saved_bytes(m, f)), dtype=torch.uint8, device=DEV)
+    ws = torch.empty(int(L.scao_gated_ff_workspace_bytes(m, d, f, 3)), dtype=torch.uint8, device=DEV)
+    dh = randn(m, f, seed=4)
+    a = _lib.GatedFfArgs()
+    a.x, a.w_gate, a.w_up, a.dh = (t.data_ptr() for t in (x, wg, wu, dh))
+    a.saved, a.workspace = saved.data_ptr(), ws.data_ptr()
+    a.ldx = a.ldg = a.ldu = ld
+    a.lddh, a.rows, a.d, a.ff, a.dtype, a.act = f, m, d, f, _lib.BF16, 0
+    bufs = {k: torch.full((n + 1024,), 7.0, dtype=torch.bfloat16, device=DEV)
+            for k, n in (("h", m * f), ("dx", m * d), ("dw_gate", f * d), ("dw_up", f * d))}
+    for (k, b), off in zip(bufs.items(), at):
+        setattr(a, k, b[512 + off:].data_ptr())
+    assert L.scao_gated_ff_forward(ctypes.byref(a), stream) == 0
+    assert L.scao_gated_ff_backward(ctypes.byref(a), stream) == 0
+    ins = [v[:, :d].detach().requires_grad_() for v in (x, wg, wu)]
+    h = gated_ff(*ins)
+    for (k, b), off, want in zip(bufs.items(), at, [h, *torch.autograd.grad(h, ins, dh)]):
+        n, lo = want.numel(), 512 + off
+        assert (b[:lo] == 7).all() and (b[lo + n:] == 7).all(), k
+        assert torch.equal(b[lo:lo + n], want.detach().reshape(-1)), k
