@@ -456,9 +456,10 @@ SCAO_API int scao_rotary(const ScaoRotary* args, void* stream);
 /* Gated feed-forward product h = act(x Wg^T) * (x Wu^T) of 16-bit matrices
  * (SCAO_BF16 / SCAO_F16), x: rows x d, Wg and Wu: ff x d, h: rows x ff, with
  * 32-bit sums.  x, w_gate, w_up start on 16 bytes and have row pitches ldx,
- * ldg, ldu that are multiples of 8 values; h, dx, dw_gate, dw_up are packed.
- * `saved` (scao_gated_ff_saved_bytes; null if no gradient will be taken)
- * keeps what backward reads.  backward: from dh (row pitch lddh) to dx and to
+ * ldg, ldu that are multiples of 8 values; h, dx, dw_gate, dw_up are packed
+ * and, like dh, may start at any value.
+ * `saved` (scao_gated_ff_saved_bytes, 16-byte aligned; null if no gradient
+ * will be taken) keeps what backward reads.  backward: from dh (row pitch lddh) to dx and to
  * dw_gate and dw_up (null: not wanted, the two together), with a workspace
  * of scao_gated_ff_workspace_bytes (which: 1 dx, 2 dw, 3 both), 16-byte
  * aligned.  pack: copies up to three matrices, rows {source, copy, rows,

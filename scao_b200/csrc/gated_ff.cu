@@ -1186,6 +1186,9 @@ bool operands_ok(const ScaoGatedFf* f) {
            f->ldx >= (f->rows ? f->d : 0) && f->ldg >= f->d && f->ldu >= f->d;
 }
 
+// 16-bit values at their own alignment
+bool even(const void* p) { return ((uintptr_t)p & 1) == 0; }
+
 }  // namespace
 
 extern "C" int* scao_gated_ff_status_word(void) { return status_word(); }
@@ -1228,7 +1231,7 @@ extern "C" int scao_gated_ff_pack(const int64_t* table, int n, void* stream) {
 extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
     if (!operands_ok(f)) return SCAO_ERR_ARG;
     if (f->rows == 0) return SCAO_OK;
-    if (!f->h) return SCAO_ERR_ARG;
+    if (!f->h || !even(f->h) || ((uintptr_t)f->saved & 15)) return SCAO_ERR_ARG;
     if (int rc = take_status()) return rc;
     const cudaStream_t st = (cudaStream_t)stream;
     if (!f->saved && plan_skinny(f->rows, f->d, f->ff)) {
@@ -1267,7 +1270,8 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
 
 extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
     if (!operands_ok(f) || f->rows == 0 || !f->saved || !f->dh || f->lddh < 0 || !f->workspace ||
-        ((uintptr_t)f->workspace & 15) || (!f->dw_gate != !f->dw_up) || up(f->ff, 128) > 65535)
+        ((uintptr_t)f->workspace & 15) || ((uintptr_t)f->saved & 15) || !even(f->dh) || !even(f->dx) ||
+        !even(f->dw_gate) || !even(f->dw_up) || (!f->dw_gate != !f->dw_up) || up(f->ff, 128) > 65535)
         return SCAO_ERR_ARG;
     if (int rc = take_status()) return rc;
     const cudaStream_t st = (cudaStream_t)stream;

@@ -79,6 +79,14 @@ def _forward(x, w_gate, w_up, act, train):
 def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w, copies):
     """(dx, dw_gate, dw_up), None where not needed."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
+    # hooks may have moved what was saved
+    like, kept = (dh.get_device(), dh.dtype), [x, w_gate, w_up, saved, *(c for c in copies if c is not None)]
+    if any((t.get_device(), t.dtype) != like for t in kept) or dh.shape != (rows, ff) or x.shape[1] != d or \
+            w_up.shape != (ff, d) or saved.numel() != L.scao_gated_ff_saved_bytes(rows, ff) >> 1 or \
+            any(c is not None and c.shape != (t.shape[0], (d + 63) & ~63) for t, c in zip(kept, copies)):
+        raise RuntimeError("gated_ff: a saved tensor came back with another size, type or device")
+    if saved.data_ptr() & 15 or not saved.is_contiguous():
+        saved = saved.clone(memory_format=torch.contiguous_format)
     dx = x.new_empty((rows, d)) if need_x else None
     new = x.new_empty if rows else x.new_zeros
     dwg, dwu = (new((ff, d)), new((ff, d))) if need_w else (None, None)

@@ -178,6 +178,7 @@ class _Turn(torch.autograd.Function):
     def forward(ctx, how, positions, q, k):
         ctx.how = how
         if positions is not None:
+            ctx.places = (positions.get_device(), positions.dtype, positions.shape)
             ctx.save_for_backward(positions)
         ctx.set_materialize_grads(False)
         rotary, inverse, start, index = how
@@ -188,6 +189,8 @@ class _Turn(torch.autograd.Function):
         rotary, inverse, start, index = ctx.how
         saved = ctx.saved_tensors
         positions = saved[0] if saved else None
+        if positions is not None and (positions.get_device(), positions.dtype, positions.shape) != ctx.places:
+            raise RuntimeError("rotary: the positions came back with another size, type or device")
         _, _, need_q, need_k = ctx.needs_input_grad
         gq, gk = gq if need_q else None, gk if need_k else None
         if torch.is_grad_enabled() or _followed():          # differentiable again

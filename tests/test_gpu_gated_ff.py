@@ -749,3 +749,30 @@ def test_results_anywhere(at, m, d, f):
         n, lo = want.numel(), 512 + off
         assert (b[:lo] == 7).all() and (b[lo + n:] == 7).all(), k
         assert torch.equal(b[lo:lo + n], want.detach().reshape(-1)), k
+
+
+@pytest.mark.parametrize("d", [64, 61])
+@pytest.mark.parametrize("m", [5, 200])
+def test_saved_tensor_hooks(m, d):
+    """Hooks may hand back what was saved anywhere in memory; of another size, type or
+    device it is refused."""
+    ins = [v.requires_grad_() for v in inputs(m, d, 48, torch.bfloat16)]
+    dh = randn(m, 48, seed=5)
+    want = torch.autograd.grad(gated_ff(*ins), ins, dh)
+
+    def through(unpack):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            h = gated_ff(*ins)
+        return torch.autograd.grad(h, ins, dh)
+
+    def moved(t, by):
+        buf = torch.empty(t.numel() + 16, dtype=t.dtype, device=DEV)
+        return buf[by:by + t.numel()].view(t.shape).copy_(t)
+
+    for by in (1, 2, 4, 7):
+        assert all(torch.equal(a, b) for a, b in zip(through(lambda t: moved(t, by)), want))
+    spread = lambda t: torch.stack([t, t], -1)[..., 0]  # noqa: E731
+    assert all(torch.equal(a, b) for a, b in zip(through(spread), want))
+    for bad in (lambda t: t.cpu(), lambda t: t.float(), lambda t: t[:t.shape[0] - 1]):
+        with pytest.raises(RuntimeError, match="another size, type or device"):
+            through(bad)

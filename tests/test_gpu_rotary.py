@@ -266,3 +266,20 @@ def test_traces(grad):
         assert torch.equal(torch.autograd.grad(y.sum(), other)[0], torch.autograd.grad(want.sum(), other)[0])
         with pytest.raises(RuntimeError, match="cannot be traced"):
             make_fx(call)(randn(1, 2, 5, 16).requires_grad_(grad))
+
+
+def test_saved_tensor_hooks():
+    """Positions that hooks hand back on another device, in another type or size are refused."""
+    r, ids = Rotary(16), torch.arange(5, device=DEV)
+    q = randn(1, 2, 5, 16).requires_grad_()
+    (want,) = torch.autograd.grad(r(q, positions=ids), q, torch.ones_like(q))
+
+    def through(unpack):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = r(q, positions=ids)
+        return torch.autograd.grad(y, q, torch.ones_like(q))[0]
+
+    assert torch.equal(through(lambda t: t.clone()), want)
+    for bad in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t[:4]):
+        with pytest.raises(RuntimeError, match="another size, type or device"):
+            through(bad)

@@ -227,6 +227,27 @@ def test_gated_ff_c_entry_checks():
     assert L.scao_gated_ff_pack(t.buffer_info()[0], 0, None) == 1
 
 
+def test_gated_ff_c_entry_alignment():
+    """Addresses that the kernels cannot read or write are refused: values of 16 bits at odd
+    bytes, what is kept for the gradient off its 16 bytes."""
+    L = _lib.lib()
+    good = dict(x=4096, w_gate=4096, w_up=4096, h=4096, saved=4096, dh=4096, dx=4096, dw_gate=4096, dw_up=4096,
+                workspace=4096, ldx=8, ldg=8, ldu=8, lddh=5, rows=3, d=8, ff=5, dtype=_lib.BF16, act=0)
+
+    def call(f, **kw):
+        a = _lib.GatedFfArgs()
+        for k, v in {**good, **kw}.items():
+            setattr(a, k, v)
+        return f(ctypes.byref(a), None)
+
+    for at in (4097, 4098, 4100, 4104):
+        assert call(L.scao_gated_ff_forward, saved=at) == 1
+        assert call(L.scao_gated_ff_backward, saved=at) == 1
+    assert call(L.scao_gated_ff_forward, h=4097) == 1
+    for k in ("dh", "dx", "dw_gate", "dw_up"):
+        assert call(L.scao_gated_ff_backward, **{k: 4097}) == 1, k
+
+
 # ----------------------------------------------------------------- the model
 @pytest.mark.parametrize("kw", [dict(mlp="moe"), dict(positions="none"), dict(n_kv_head=5), dict(n_kv_head=0)])
 def test_gpt_config_refuses(kw):
