@@ -682,60 +682,61 @@ ff_pointwise_kernel(const unsigned char* __restrict__ saved, const uint16_t* __r
          i += (int64_t)gridDim.x * gridDim.y * PT)
         count[i] = 0;
     const int cb = (cols + 127) >> 7, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c = blockIdx.y * 128 + (warp & 1) * 64 + (lane & 3) * 16;
-    if (c >= cols) return;
-    for (int i = (warp >> 1) * 8 + (lane >> 2); i < span; i += 32) {
-        const int r = blockIdx.x * span + i;
-        if (r >= rows) break;
-        const unsigned char* p = saved + saved_off(r, c, cb);
-        uint4 gw[3], uw[3];
+    // once round, unless there are more blocks of columns than a grid has places
+    for (int c = blockIdx.y * 128 + (warp & 1) * 64 + (lane & 3) * 16; c < cols; c += gridDim.y * 128) {
+        for (int i = (warp >> 1) * 8 + (lane >> 2); i < span; i += 32) {
+            const int r = blockIdx.x * span + i;
+            if (r >= rows) break;
+            const unsigned char* p = saved + saved_off(r, c, cb);
+            uint4 gw[3], uw[3];
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
-            gw[k] = *(const uint4*)(p + k * SAVED_PLANE);
-            uw[k] = *(const uint4*)(p + SAVED_BLOCK + k * SAVED_PLANE);
-        }
-        const uint16_t* d = dh + r * lddh + c;
-        uint32_t y[8];
-        if (vec) {
-            const bool all = c + 8 < cols;
-            const uint4 a = *(const uint4*)d, b = all ? *(const uint4*)(d + 8) : make_uint4(0, 0, 0, 0);
-            y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w;
-            y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                y[k] = (c + 2 * k < cols ? (uint32_t)d[2 * k] : 0) |
-                       (c + 2 * k + 1 < cols ? (uint32_t)d[2 * k + 1] << 16 : 0);
-        }
-        const uint32_t gq[12] = {gw[0].x, gw[0].y, gw[0].z, gw[0].w, gw[1].x, gw[1].y,
-                                 gw[1].z, gw[1].w, gw[2].x, gw[2].y, gw[2].z, gw[2].w};
-        const uint32_t uq[12] = {uw[0].x, uw[0].y, uw[0].z, uw[0].w, uw[1].x, uw[1].y,
-                                 uw[1].z, uw[1].w, uw[2].x, uw[2].y, uw[2].z, uw[2].w};
-        uint32_t og[8], ou[8];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float g[4], u[4], a[4], b[4], z[4];
-            restore4(gq[3 * k], gq[3 * k + 1], gq[3 * k + 2], g);
-            restore4(uq[3 * k], uq[3 * k + 1], uq[3 * k + 2], u);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t bits = y[2 * k + (e >> 1)] >> (16 * (e & 1)) & 0xffff;
-                z[e] = dtype == SCAO_BF16 ? bf16_bits_to_f(bits) : f16_bits_to_f(bits);
-                ff_act_grad<ACT>(g[e], a[e], b[e]);
+            for (int k = 0; k < 3; ++k) {
+                gw[k] = *(const uint4*)(p + k * SAVED_PLANE);
+                uw[k] = *(const uint4*)(p + SAVED_BLOCK + k * SAVED_PLANE);
             }
+            const uint16_t* d = dh + r * lddh + c;
+            uint32_t y[8];
+            if (vec) {
+                const bool all = c + 8 < cols;
+                const uint4 a = *(const uint4*)d, b = all ? *(const uint4*)(d + 8) : make_uint4(0, 0, 0, 0);
+                y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w;
+                y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-                ou[2 * k + e / 2] = pack2(z[e] * a[e], z[e + 1] * a[e + 1], dtype);
-                og[2 * k + e / 2] = pack2(z[e] * u[e] * b[e], z[e + 1] * u[e + 1] * b[e + 1], dtype);
+                for (int k = 0; k < 8; ++k)
+                    y[k] = (c + 2 * k < cols ? (uint32_t)d[2 * k] : 0) |
+                           (c + 2 * k + 1 < cols ? (uint32_t)d[2 * k + 1] << 16 : 0);
             }
+            const uint32_t gq[12] = {gw[0].x, gw[0].y, gw[0].z, gw[0].w, gw[1].x, gw[1].y,
+                                     gw[1].z, gw[1].w, gw[2].x, gw[2].y, gw[2].z, gw[2].w};
+            const uint32_t uq[12] = {uw[0].x, uw[0].y, uw[0].z, uw[0].w, uw[1].x, uw[1].y,
+                                     uw[1].z, uw[1].w, uw[2].x, uw[2].y, uw[2].z, uw[2].w};
+            uint32_t og[8], ou[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float g[4], u[4], a[4], b[4], z[4];
+                restore4(gq[3 * k], gq[3 * k + 1], gq[3 * k + 2], g);
+                restore4(uq[3 * k], uq[3 * k + 1], uq[3 * k + 2], u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t bits = y[2 * k + (e >> 1)] >> (16 * (e & 1)) & 0xffff;
+                    z[e] = dtype == SCAO_BF16 ? bf16_bits_to_f(bits) : f16_bits_to_f(bits);
+                    ff_act_grad<ACT>(g[e], a[e], b[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    ou[2 * k + e / 2] = pack2(z[e] * a[e], z[e + 1] * a[e + 1], dtype);
+                    og[2 * k + e / 2] = pack2(z[e] * u[e] * b[e], z[e + 1] * u[e + 1] * b[e + 1], dtype);
+                }
+            }
+            // dg and du have a pitch of whole lines: this may write past `cols` within it, where the
+            // products read nothing
+            uint16_t *pg = dg + r * ldg + c, *pu = du + r * ldg + c;
+            *(uint4*)pg = make_uint4(og[0], og[1], og[2], og[3]);
+            *(uint4*)(pg + 8) = make_uint4(og[4], og[5], og[6], og[7]);
+            *(uint4*)pu = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+            *(uint4*)(pu + 8) = make_uint4(ou[4], ou[5], ou[6], ou[7]);
         }
-        // dg and du have a pitch of whole lines: this may write past `cols` within it, where the
-        // products read nothing
-        uint16_t *pg = dg + r * ldg + c, *pu = du + r * ldg + c;
-        *(uint4*)pg = make_uint4(og[0], og[1], og[2], og[3]);
-        *(uint4*)(pg + 8) = make_uint4(og[4], og[5], og[6], og[7]);
-        *(uint4*)pu = make_uint4(ou[0], ou[1], ou[2], ou[3]);
-        *(uint4*)(pu + 8) = make_uint4(ou[4], ou[5], ou[6], ou[7]);
     }
 }
 
@@ -1271,7 +1272,7 @@ extern "C" int scao_gated_ff_forward(const ScaoGatedFf* f, void* stream) {
 extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
     if (!operands_ok(f) || f->rows == 0 || !f->saved || !f->dh || f->lddh < 0 || !f->workspace ||
         ((uintptr_t)f->workspace & 15) || ((uintptr_t)f->saved & 15) || !even(f->dh) || !even(f->dx) ||
-        !even(f->dw_gate) || !even(f->dw_up) || (!f->dw_gate != !f->dw_up) || up(f->ff, 128) > 65535)
+        !even(f->dw_gate) || !even(f->dw_up) || (!f->dw_gate != !f->dw_up))
         return SCAO_ERR_ARG;
     if (int rc = take_status()) return rc;
     const cudaStream_t st = (cudaStream_t)stream;
@@ -1292,7 +1293,8 @@ extern "C" int scao_gated_ff_backward(const ScaoGatedFf* f, void* stream) {
         // rows of a block: 128, fewer where that would leave SMs without one
         int span = 128;
         while (span > 32 && (int64_t)up(f->rows, span) * up(f->ff, 128) < 4 * scao_sm_count()) span >>= 1;
-        kernel<<<dim3(up(f->rows, span), up(f->ff, 128)), PT, 0, st>>>(
+        const int across = up(f->ff, 128);
+        kernel<<<dim3(up(f->rows, span), across < 65535 ? across : 65535), PT, 0, st>>>(
             (const unsigned char*)f->saved, (const uint16_t*)f->dh, f->lddh, dg, du, ld, f->rows, f->ff, f->dtype, vec,
             span, (int*)(ws + space.count), (int)p.counts);
         SCAO_CHECK_LAUNCH();

@@ -776,3 +776,12 @@ def test_saved_tensor_hooks(m, d):
     for bad in (lambda t: t.cpu(), lambda t: t.float(), lambda t: t[:t.shape[0] - 1]):
         with pytest.raises(RuntimeError, match="another size, type or device"):
             through(bad)
+
+
+def test_widest():
+    """The largest inner width: more blocks of columns than a grid has places in that direction."""
+    f = (1 << 23) - 1
+    x, wg, wu = inputs(2, 8, f, torch.bfloat16)
+    check(x, wg, wu, "silu", True)
+    with pytest.raises(ValueError, match="widths below"):
+        gated_ff(x, wg.new_empty(f + 1, 8), wu.new_empty(f + 1, 8))
