@@ -6,7 +6,7 @@ and return the norm as a float32 scalar on the gradients' device; nothing waits 
 the GPU.  Gradients may mix float32, bfloat16 and float16, sizes and alignments.
 Sums are held in 64 bits over the whole range of float32, the same inputs give the
 same bits, and each scaled value is rounded once.  Gradients within the threshold are
-not written.  CUDA tensors of one device only; errors raise.
+not written (strided ones that do not fill a range of memory are: with their own values).  CUDA tensors of one device only; errors raise.
 """
 from __future__ import annotations
 
@@ -22,6 +22,7 @@ from .cuda import _CODE, _followed, _launch
 
 _KIND = {1.0: 0, 2.0: 1, math.inf: 2}
 _DTYPES = set(_CODE)
+SHARED = "two gradients share memory: each can be scaled only once"
 _DTYPE, _LAYOUT, _GRAD = attrgetter("dtype"), attrgetter("layout"), attrgetter("grad")
 
 
@@ -35,6 +36,53 @@ def _layout(t):
         dense = dense and stride == expected
         expected += stride * (size - 1)
     return dense, False
+
+
+def _places(t):
+    """Where a tensor's bytes lie: (first address, [(count, stride in bytes)] from the widest
+    stride on, bytes of an unbroken run, bytes from the first to behind the last)."""
+    size = run = t.element_size()
+    steps = []
+    for stride, n in sorted((st * size, n) for n, st in zip(t.shape, t.stride()) if n != 1):
+        if not steps and stride == run:
+            run *= n
+        else:
+            steps.append((n, stride))
+    return t.data_ptr(), steps[::-1], run, run + sum((n - 1) * st for n, st in steps)
+
+
+def _meet(p, a, run_a, span_a, q, b, run_b, span_b):
+    """Whether two tensors, neither of which overlaps itself, share a byte (``_places`` of
+    both).  A step's span is at most its stride, so with equal strides only the neighbouring
+    shifts of one against the other can meet; else the wider steps are taken one by one, where
+    they reach the other tensor."""
+    if p + span_a <= q or q + span_b <= p:
+        return False
+    if not a and not b:
+        return True
+    if not a or (b and b[0][1] > a[0][1]):
+        p, a, run_a, span_a, q, b, run_b, span_b = q, b, run_b, span_b, p, a, run_a, span_a
+    n, stride = a[0]
+    a, span_a = a[1:], span_a - (n - 1) * stride
+    low, high = 0, n - 1
+    if b and b[0][1] == stride:
+        m, b, span_b = b[0][0], b[1:], span_b - (b[0][0] - 1) * stride
+        low -= m - 1
+    # steps i for which [p + i stride, + span_a) meets [q, q + span_b)
+    low, high = max(low, (q - p - span_a) // stride + 1), min(high, (q + span_b - p - 1) // stride)
+    return any(_meet(p + i * stride, a, run_a, span_a, q, b, run_b, span_b) for i in range(low, high + 1))
+
+
+def _refuse_sharing(tensors, strided):
+    """Raises where one of the ``strided`` tensors (by number) shares memory with another."""
+    places = sorted(((*_places(t), i in strided) for i, t in enumerate(tensors) if t.numel()),
+                    key=lambda x: x[0])
+    near = []
+    for p, steps, run, span, loose in places:
+        near = [x for x in near if x[0] + x[3] > p]
+        if any((loose or x[4]) and _meet(*x[:4], p, steps, run, span) for x in near):
+            raise ValueError(SHARED)
+        near.append((p, steps, run, span, loose))
 
 
 def _refuse(tensors):
@@ -62,7 +110,7 @@ def _table(tensors, write):
             set(map(_LAYOUT, tensors)) != {torch.strided}:
         _refuse(tensors)
     codes = [_CODE[dtypes.pop()]] * n if len(dtypes) == 1 else [_CODE[t.dtype] for t in tensors]
-    packed = []
+    packed, strided = [], set()
     if not all(map(get.is_contiguous, tensors)):
         tensors = list(tensors)
         for i, t in enumerate(tensors):
@@ -73,8 +121,12 @@ def _table(tensors, write):
                 raise ValueError("a gradient shares memory with itself (an expanded view): "
                                  "it cannot be scaled in place")
             if not dense:
-                tensors[i] = t.detach().contiguous()
-                packed.append((t, tensors[i]))
+                strided.add(i)
+        if write and strided:
+            _refuse_sharing(tensors, strided)
+        for i in strided:
+            t, tensors[i] = tensors[i], tensors[i].detach().contiguous()
+            packed.append((t, tensors[i]))
     rows = [0] * (3 * n)
     rows[0::3] = list(map(get.data_ptr, tensors))
     rows[1::3] = list(map(get.numel, tensors))
@@ -83,7 +135,7 @@ def _table(tensors, write):
     if write:
         rc = _lib.lib().scao_grads_overlap(table.buffer_info()[0], n)
         if rc == 1:
-            raise ValueError("two gradients share memory: each can be scaled only once")
+            raise ValueError(SHARED)
         _lib.check(rc, "scao_grads_overlap")
     if not tensors[0].is_cuda:
         raise RuntimeError("scao_b200: gradients must be CUDA tensors (no CPU path)")

@@ -219,3 +219,20 @@ def test_train_step_clips():
     ob.step()
     for p, q in zip(a.parameters(), b.parameters()):
         assert torch.equal(p, q)
+
+
+def test_column_halves():
+    """Gradients that interleave in memory without sharing are clipped as any; sharing ones are
+    refused and stay as they are."""
+    base = torch.randn(64, 100, device=DEV)
+    check([base[:, :50], base[:, 50:]], 2, 0.5)
+    check([base[::2], base[1::2, 3:9]], math.inf, 0.01)
+    keep = base.clone()
+    for a, b in ((base[:, :51], base[:, 50:]), (base, base[:, ::2])):
+        with pytest.raises(ValueError, match="share memory"):
+            clip_grad_norm_(params_of([a, b]), 1e-3)
+        with pytest.raises(ValueError, match="share memory"):
+            clip_grads_with_norm_(params_of([a, b]), 1e-3, torch.ones((), device=DEV))
+    assert torch.equal(base, keep)
+    want = norm64([base, base[:, ::2]], 2)              # a norm only reads
+    assert abs(get_total_norm([base, base[:, ::2]]).item() - want) <= 2.0 ** -18 * want

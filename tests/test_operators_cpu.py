@@ -58,6 +58,75 @@ def test_clip_refuses_shared_memory():
         clip_grad_norm_([param(base[:10]), param(base[10:])], 1.0)
 
 
+@pytest.mark.parametrize("a,b,shares", [
+    (lambda x: x[:, :5], lambda x: x[:, 3:], True), (lambda x: x, lambda x: x[:, ::2], True),
+    (lambda x: x[:, :5], lambda x: x[:, 5:], False), (lambda x: x[:, ::2], lambda x: x[:, 1::2], False),
+    (lambda x: x[:, ::2], lambda x: x[:, ::3], True), (lambda x: x[::2], lambda x: x[1::2, 2:5], False),
+    (lambda x: x[::2], lambda x: x[1::3], True), (lambda x: x[1::4, :3], lambda x: x[::2], False),
+    (lambda x: x[2:4], lambda x: x[:, 1:3], True), (lambda x: x[9:], lambda x: x[:9, 1:3], False),
+    (lambda x: x[:, 1], lambda x: x[7], True), (lambda x: x[:, 1].bfloat16, lambda x: x[:, 1], False)])
+def test_clip_refuses_shared_memory_of_views(a, b, shares):
+    base = torch.ones(12, 8)
+    a, b = a(base), b(base)
+    pair = [param(v() if callable(v) else v) for v in (a, b)]
+    for grads in (pair, pair[::-1], [param(torch.ones(3)), *pair]):
+        with pytest.raises(ValueError if shares else RuntimeError, match="share memory" if shares else "CUDA"):
+            clip_grad_norm_(grads, 1.0)
+
+
+def test_sharing_of_views_is_exact():
+    """Against the sets of the bytes, for many pairs of views."""
+    import random
+
+    from scao_b200.clip import _meet, _places
+    rng = random.Random(5)
+    base = torch.zeros(600, dtype=torch.float32)
+    half = base.view(torch.bfloat16)
+
+    def view():
+        flat = rng.choice([base, half])
+        while True:
+            shape = [rng.choice([1, 2, 3, 4, 7]) for _ in range(rng.randint(1, 3))]
+            stride, need = [], rng.choice([1, 1, 2, 3, 5])
+            for n in shape:
+                stride.append(need)
+                need = need * n + rng.choice([0, 0, 1, 4])
+            order = list(range(len(shape)))
+            rng.shuffle(order)
+            shape, stride = [shape[i] for i in order], [stride[i] for i in order]
+            if need < 500:
+                return flat.as_strided(shape, stride, rng.randrange(40 * flat.numel() // 600))
+
+    def bytes_of(t):
+        at = torch.zeros(t.shape, dtype=torch.long) + t.data_ptr()
+        for i, (n, st) in enumerate(zip(t.shape, t.stride())):
+            at = at + (torch.arange(n) * st * t.element_size()).view([-1 if k == i else 1 for k in range(t.dim())])
+        return {int(x) + k for x in at.flatten() for k in range(t.element_size())}
+
+    found = [0, 0]
+    for _ in range(3000):
+        a, b = view(), view()
+        if _layout(a)[1] or _layout(b)[1]:
+            continue
+        want = not bytes_of(a).isdisjoint(bytes_of(b))
+        assert _meet(*_places(a), *_places(b)) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride())
+        found[want] += 1
+    assert min(found) > 500, found
+
+
+def test_sharing_of_long_views_is_quick():
+    """Two halves of the columns of a tall matrix: a few steps, not one a row."""
+    import time
+    base = torch.zeros(1 << 20, 8)
+    pair = [param(base[:, :4]), param(base[:, 4:])]
+    with pytest.raises(RuntimeError, match="CUDA"):
+        clip_grad_norm_(pair, 1.0)
+    from scao_b200.clip import _refuse_sharing
+    start = time.perf_counter()
+    _refuse_sharing([p.grad for p in pair], {0, 1})
+    assert time.perf_counter() - start < 0.1
+
+
 def test_clip_refuses_forward_mode():
     from torch.autograd import forward_ad
     with forward_ad.dual_level():
