@@ -416,7 +416,8 @@ SCAO_API int scao_divc_check(const float* x, const float* c, int n, int* mismatc
 /* Global norm of many gradients and clipping by it.  `table` (host): n rows
  * of {device address, number of values, dtype}.  kind: the norm.  The norm of
  * no values is 0; a NaN anywhere makes it NaN.  Accumulated in 64 bits,
- * written as one float; the same inputs give the same bits.                */
+ * written as one float; the same inputs give the same bits.  The workspace
+ * (scao_grad_norm_workspace_bytes) starts on 8 bytes.                      */
 #define SCAO_NORM_1 0
 #define SCAO_NORM_2 1
 #define SCAO_NORM_INF 2

@@ -371,6 +371,8 @@ int norm_and_clip(const int64_t* table, int n, int kind, bool clip, double max_n
                   const float* total_in, float* total_out, cudaStream_t st) {
     if (kind < SCAO_NORM_1 || kind > SCAO_NORM_INF) return SCAO_ERR_ARG;
     if (clip && !(max_norm >= 0)) return SCAO_ERR_ARG;
+    if ((uintptr_t)partial % sizeof(double) || ((uintptr_t)total_in | (uintptr_t)total_out) % sizeof(float))
+        return SCAO_ERR_ARG;
     try {
         std::vector<Grad> g;
         if (!read_table(table, n, g)) return SCAO_ERR_ARG;

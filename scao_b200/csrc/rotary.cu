@@ -337,7 +337,8 @@ int launch_layout(RotArgs& A, bool inter, int nv, int row, cudaStream_t st) {
 
 extern "C" int scao_rotary(const ScaoRotary* r, void* stream) {
     if (!r || r->dtype < SCAO_F32 || r->dtype > SCAO_F16 || r->dim < 2 || (r->dim & 1) ||
-        r->dim > 2 * RMAX || r->head_dim < r->dim || r->batch < 0 || r->len < 0 || !r->turns)
+        r->dim > 2 * RMAX || r->head_dim < r->dim || r->batch < 0 || r->len < 0 || !r->turns ||
+        (uintptr_t)r->positions % (r->positions_64 ? 8 : 4))
         return SCAO_ERR_ARG;
     RotArgs A;
     A.T = r->len;

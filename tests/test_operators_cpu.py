@@ -170,6 +170,24 @@ def test_clip_c_entry_checks():
     assert L.scao_grad_norm_workspace_bytes(1) <= L.scao_grad_norm_workspace_bytes(5000)
 
 
+def test_c_entries_refuse_misaligned_addresses():
+    """Scalars, workspaces and positions that do not lie as their types need."""
+    L = _lib.lib()
+    t = array("q", (4096, 5, 0))
+    at = t.buffer_info()[0]
+    for ws, total in ((4100, 4096), (4096, 4098)):
+        assert L.scao_grad_norm(at, 1, 1, ws, total, None) == 1
+        assert L.scao_grad_norm_clip(at, 1, 1, 1.0, ws, total, None) == 1
+    assert L.scao_grad_clip(at, 1, 1.0, 4097, None) == 1
+    turns = (ctypes.c_double * 4)(*[0.1] * 4)
+    for pos, wide in ((4098, 0), (4097, 0), (4100, 1)):
+        a = _lib.RotaryArgs()
+        a.turns, a.dim, a.head_dim, a.batch, a.len, a.dtype = ctypes.addressof(turns), 8, 8, 1, 1, 0
+        a.heads[0], a.positions, a.positions_64 = 1, pos, wide
+        a.src[0] = a.dst[0] = 4096
+        assert L.scao_rotary(ctypes.byref(a), None) == 1, (pos, wide)
+
+
 @pytest.mark.parametrize("pre_dispatch", [False, True])
 def test_fx_traces_are_refused(pre_dispatch):
     from torch.fx.experimental.proxy_tensor import make_fx
