@@ -482,6 +482,11 @@ typedef struct {
 } ScaoGatedFf;
 SCAO_API int64_t scao_gated_ff_saved_bytes(int rows, int ff);
 SCAO_API int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff, int which);
+/* What a call will launch (host only): {tiles: 0 of 128 x 128 by a CTA, 1 of
+ * 256 x 256 and 2 of 512 x 256 by two; work items; cuts of dx's and of dw's
+ * contraction; CTAs or pairs that share the items}.  which: 0 a forward pass
+ * that keeps what the gradient reads, else as for the workspace.           */
+SCAO_API int scao_gated_ff_plan(int rows, int d, int ff, int which, int32_t* out);
 SCAO_API int scao_gated_ff_pack(const int64_t* table, int n, void* stream);
 SCAO_API int* scao_gated_ff_status_word(void);
 SCAO_API int scao_gated_ff_forward(const ScaoGatedFf* args, void* stream);

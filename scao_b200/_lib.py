@@ -168,6 +168,7 @@ SIGNATURES = {
     "scao_rotary": (C.c_int, [_P, _P]),
     "scao_gated_ff_saved_bytes": (C.c_int64, [C.c_int, C.c_int]),
     "scao_gated_ff_workspace_bytes": (C.c_int64, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "scao_gated_ff_plan": (C.c_int, [C.c_int] * 4 + [C.POINTER(C.c_int32)]),
     "scao_gated_ff_pack": (C.c_int, [_P, C.c_int, _P]),
     "scao_gated_ff_status_word": (C.POINTER(C.c_int), []),
     "scao_gated_ff_forward": (C.c_int, [_P, _P]),

@@ -1203,6 +1203,24 @@ extern "C" int64_t scao_gated_ff_workspace_bytes(int rows, int d, int ff, int wh
     return space_of(plan_backward(rows, d, ff, which & 1, which & 2), rows, ff).bytes;
 }
 
+extern "C" int scao_gated_ff_plan(int rows, int d, int ff, int which, int32_t* out) {
+    if (rows < 1 || d < 1 || ff < 1 || which < 0 || which > 3 || !out) return SCAO_ERR_ARG;
+    if (which == 0) {
+        out[0] = plan_forward(rows, d, ff);
+        out[1] = (int32_t)tiles_of(rows, ff, tile_rows(out[0]), tile_cols(out[0]) / 2);
+        out[2] = out[3] = 1;
+    } else {
+        const FfPlan& p = plan_backward(rows, d, ff, which & 1, which & 2);
+        if (p.us < 0) return SCAO_ERR_ARG;
+        out[0] = p.shape;
+        out[1] = p.dx_items + p.dw_items;
+        out[2] = p.dx.splits;
+        out[3] = p.dw.splits;
+    }
+    out[4] = group_count(out[0]);
+    return SCAO_OK;
+}
+
 extern "C" int scao_gated_ff_pack(const int64_t* table, int n, void* stream) {
     if (!table || n < 1 || n > 3) return SCAO_ERR_ARG;
     FfPack P;

@@ -13,6 +13,7 @@ import math
 import pytest
 import torch
 
+from gated_ff_shapes import PATHS, plan
 from scao_b200 import GatedFeedForward, _lib, gated_ff, gpt
 
 pytestmark = pytest.mark.gpu
@@ -785,3 +786,20 @@ def test_widest():
     check(x, wg, wu, "silu", True)
     with pytest.raises(ValueError, match="widths below"):
         gated_ff(x, wg.new_empty(f + 1, 8), wu.new_empty(f + 1, 8))
+
+
+@pytest.mark.parametrize("sizes", list(PATHS))
+def test_tile_paths(sizes):
+    """Every tile with several items a CTA or pair, and whole and cut contractions, for both
+    gradient products together and for each alone."""
+    assert [(w, *plan(*sizes, w)) for w, *_ in PATHS[sizes]] == PATHS[sizes]
+    x, wg, wu = inputs(*sizes, torch.float16 if sizes[2] % 2 else torch.bfloat16)
+    check(x, wg, wu, "silu", True)
+    dh = randn(sizes[0], sizes[2], t=x.dtype, seed=7, scale=0.1)
+    want = backward64(x, wg, wu, dh, "silu")
+    for which in (1, 2):
+        ins = [v.detach().requires_grad_(which == (1 if i == 0 else 2)) for i, v in enumerate((x, wg, wu))]
+        need = [v for v in ins if v.requires_grad]
+        grads = torch.autograd.grad(gated_ff(*ins), need, dh)
+        for got, (value, err) in zip(grads, want[:1] if which == 1 else want[1:]):
+            close(got, value, err)

@@ -8,6 +8,7 @@ from array import array
 import pytest
 import torch
 
+from gated_ff_shapes import PAIR, PATHS, SINGLE, TALL, plan
 from scao_b200 import (GatedFeedForward, Rotary, RotaryScaling, _lib, clip_grad_norm_,
                        clip_grads_with_norm_, gated_ff, get_total_norm, gpt)
 from scao_b200.clip import _layout
@@ -333,6 +334,28 @@ def test_gated_ff_c_entry_alignment():
     assert call(L.scao_gated_ff_forward, h=4097) == 1
     for k in ("dh", "dx", "dw_gate", "dw_up"):
         assert call(L.scao_gated_ff_backward, **{k: 4097}) == 1, k
+
+
+def test_gated_ff_tile_paths():
+    """The sizes of the GPU tests still reach the tile paths that they stand for; together all."""
+    seen = set()
+    for sizes, paths in PATHS.items():
+        for which, *want in paths:
+            assert plan(*sizes, which) == tuple(want), (sizes, which)
+            tile, dx, dw, several = want
+            seen.add((which > 0, tile, several))
+            if which:
+                seen.add((tile, "dx", dx > 1))
+                seen.add((tile, "dw", dw > 1))
+    assert {(False, t, True) for t in range(3)} | {(True, PAIR, True), (True, TALL, True)} <= seen
+    assert {(PAIR, "dx", True), (PAIR, "dw", True), (SINGLE, "dx", True), (SINGLE, "dw", True)} <= seen
+
+
+def test_gated_ff_plan_checks():
+    L, out = _lib.lib(), (ctypes.c_int32 * 5)()
+    for args in ((0, 8, 8, 3), (8, 0, 8, 3), (8, 8, -1, 0), (8, 8, 8, 4), (8, 8, 8, -1)):
+        assert L.scao_gated_ff_plan(*args, out) == 1, args
+    assert L.scao_gated_ff_plan(8, 8, 8, 3, None) == 1
 
 
 # ----------------------------------------------------------------- the model
