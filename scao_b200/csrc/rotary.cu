@@ -6,10 +6,14 @@
 // The gradient is the transposed rotation: the same kernel with -sin.
 //
 // The angle is formed in turns, as a fixed-point fraction of 64 bits: p times the
-// fraction w_j / 2 pi 2^64, of which a 64-bit product keeps exactly what is left when whole
-// turns are taken off (in 32-bit floats p w_j / 2 pi of far positions would be off by 1e-2
-// turns and more; doubles would do, at three conversions of a quarter of the rate
-// each).  Its upper 32 bits, as a signed part of a turn, go to sincospif.  The
+// fraction w_j / 2 pi 2^64, of which a 64-bit product keeps what is left when whole turns are
+// taken off (in 32-bit floats p w_j / 2 pi of far positions would be off by 1e-2 turns and
+// more; doubles would do, at three conversions of a quarter of the rate each).  What it is
+// off by is p times the error of the fraction, which comes as a double: at most 2^-55.2
+// (w_j <= 1, two roundings of 53 bits, and the cut at 2^-64).  Its upper 32 bits, as a signed
+// part of a turn, are rounded to a float for sincospif: 2^-26 of a turn, 1e-7 radian, as
+// much as one rounding of a float32 result and nothing beside those of 16-bit types (a
+// float32 result is off by 1.3 times what angles rounded only once would leave).  The
 // frequencies travel as kernel arguments (dim <= 512: 2 KB), so there is no table in
 // memory to keep or to outgrow.
 //

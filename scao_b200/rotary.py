@@ -7,10 +7,11 @@
 
 Pair j of a head at position p turns by p w_j, w_j = base^(-2j / dim); the pair is
 (2j, 2j + 1) where ``interleaved``, else (j, j + dim / 2); values from ``dim`` on pass
-through.  Forward-mode derivatives raise.  Angles are formed in 64 bits, so far positions stay exact.  Any strides with
-neighbouring values of a head next to each other are read as they are (views of a fused
-projection, (batch, length, heads, head_dim) memory).  float32, bfloat16 and float16,
-CUDA tensors of one device.
+through.  Angles are formed in 64 bits: at position p off by at most |p| 2^-55 of a turn
+(base >= 1), which up to 2^29 is no more than their rounding to 24 bits for cos and sin
+(2^-26 of a turn).  Any strides with neighbouring values of a head next to each other are
+read as they are (views of a fused projection, (batch, length, heads, head_dim) memory).
+float32, bfloat16 and float16, CUDA tensors of one device.  Forward-mode derivatives raise.
 """
 from __future__ import annotations
 

@@ -283,3 +283,22 @@ def test_saved_tensor_hooks():
     for bad in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t[:4]):
         with pytest.raises(RuntimeError, match="another size, type or device"):
             through(bad)
+
+
+@pytest.mark.parametrize("dim", [8, 128])
+@pytest.mark.parametrize("pos", [1 << 29, -(1 << 29) - 7, 1 << 33, (1 << 40) + 12345, -(1 << 45) + 1, (1 << 50) + 3])
+def test_angles_of_very_far_positions(pos, dim):
+    """Against angles in rational numbers: off by at most |p| 2^-55 of a turn on top of the
+    float32 bound at the head of this file."""
+    from fractions import Fraction
+    two_pi = Fraction(628318530717958647692528676655900576839433879875021, 10 ** 50)
+    r = Rotary(dim)
+    x = randn(1, 1, 1, dim, seed=3)
+    turns = [Fraction(float(w)) * pos / two_pi for w in r.frequencies]
+    angle = torch.tensor([float(t - math.floor(t)) for t in turns], dtype=torch.float64, device=DEV) * (2 * math.pi)
+    a, b = x.double().chunk(2, -1)
+    want = torch.cat([a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()], -1)
+    size = torch.hypot(a, b).repeat(1, 1, 1, 2)
+    tol = size * (2.0 ** -21 + 2 * math.pi * abs(pos) * 2.0 ** -55) + 2.0 ** -24 * want.abs()
+    for y in (r(x, positions=pos), r(x, positions=torch.tensor([pos], device=DEV))):
+        assert ((y.double() - want).abs() <= tol).all()
