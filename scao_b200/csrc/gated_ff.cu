@@ -17,7 +17,7 @@
 //              rounded to 16 bits as operands of the tensor cores.
 // That pass reads g and u as the forward pass kept them, in 24 bits: in 16 their rounding
 // would come beside those of dg, du and the result, and put the gradients' error at 1.8
-// instead of 1.4 roundings.
+// instead of 1.4 roundings (of either type; 32 bits would not lower it).
 //
 // Few rows without a gradient take ff_skinny_kernel.
 //
@@ -170,8 +170,9 @@ SCAO_DEV uint32_t pack2(float a, float b, int dt) {
 }
 
 // g and u as kept for the gradient: rounded to 24 bits (16 of the significand), 3 bytes a
-// value, which is 2^-8 of a 16-bit rounding and a quarter less to write and read than 32.
-// Per 128-row x 128-column block the g values, then the u values, as [16-column
+// value, which is 2^-8 of a bfloat16 rounding, 2^-5 of a float16 one, and a quarter less to
+// write and read than 32.
+// Per whole 128-row x 128-column block the g values, then the u values, as [16-column
 // group][16 bytes of its 48][row], so that a warp (a thread per row) writes 512
 // consecutive bytes.
 constexpr int SAVED_BLOCK = 128 * 128 * 3;

@@ -6,7 +6,8 @@
 (..., ff), all bfloat16 or all float16 (under CUDA autocast they are cast to its type)
 with 32-bit sums.  The activation is "silu", "gelu" or "gelu_tanh".  Both projections,
 the activation and the product are one kernel; where a gradient will be taken it also
-keeps both projections' results in 24 bits (6 bytes for each value of h).
+keeps both projections' results in 24 bits (6 bytes for each value of h, in whole blocks
+of 128 rows x 128 columns: one row keeps what 128 do).
 
 Any sizes; rows that are a multiple of 16 bytes apart are read as they lie, others are
 copied first.  ``GatedFeedForward`` is the block with its output projection.
