@@ -79,3 +79,27 @@ def test_reference_line_contract():
     assert "1 of 12 transformer layers" in cb["sample"]
     assert d["e2e"] == {"value": d["value"], "unit": "ms",
                         "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0}
+
+
+def test_without_the_reference_package(monkeypatch, tmp_path, capsys):
+    """Where baseline/_ref is missing the reference arm says so and ends well, and the
+    module names nothing that it does not define."""
+    import builtins
+    import json
+    import symtable
+    monkeypatch.setattr(bench, "ROOT", str(tmp_path))
+    monkeypatch.setattr("sys.argv", ["bench.py", "--impl", "reference", "--workload", "gpt2-small"])
+    bench.main()
+    d = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert d["impl"] == "reference" and "not installed" in d["unavailable"] and "value" not in d
+
+    def free(table):
+        for s in table.get_symbols():
+            if s.is_referenced() and s.is_global() and not s.is_assigned():
+                yield s.get_name()
+        for t in table.get_children():
+            yield from free(t)
+
+    with open(bench.__file__) as f:
+        names = set(free(symtable.symtable(f.read(), "bench.py", "exec")))
+    assert not {n for n in names if not hasattr(bench, n) and not hasattr(builtins, n)}
