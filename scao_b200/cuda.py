@@ -10,9 +10,10 @@ RuntimeError, as does any error status of the library call.
 from __future__ import annotations
 
 import torch
-from torch._C import _len_torch_dispatch_stack as _modes
-from torch._ops import _len_torch_dispatch_stack_pre_dispatch as _pre_dispatch_modes
+from torch._C import _is_tracing
+from torch._C._autograd import _top_saved_tensors_default_hooks as _hooks
 from torch.autograd import forward_ad
+from torch.fx import _symbolic_trace
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
@@ -36,7 +37,13 @@ def _followed():
     """Whether forward-mode derivatives or torch.jit.trace follow the call: they see an
     autograd function (which raises for a tangent, and which a trace calls again), but not a
     launch into a new tensor."""
-    return forward_ad._current_level >= 0 or torch._C._is_tracing()
+    return forward_ad._current_level >= 0 or _is_tracing()
+
+
+def _hooked():
+    """Whether what is saved for a gradient now goes through hooks, which may hand back
+    something else."""
+    return _hooks(False) is not None
 
 
 def _launch(what, index, fn, *args):
@@ -44,7 +51,7 @@ def _launch(what, index, fn, *args):
     handle and the device number: the stream objects of ``torch.cuda`` cost several
     microseconds, as much as a small kernel.)  An FX trace of real tensors would record
     the outputs as they were allocated and nothing that fills them."""
-    if (_modes() or _pre_dispatch_modes()) and get_proxy_mode() is not None:
+    if _symbolic_trace._is_fx_tracing_flag and get_proxy_mode() is not None:
         raise RuntimeError(f"{what} cannot be traced into an FX graph")
     if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))

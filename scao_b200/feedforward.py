@@ -14,17 +14,21 @@ copied first.  ``GatedFeedForward`` is the block with its output projection.
 """
 from __future__ import annotations
 
+import operator
 import struct
 from array import array
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
-from .cuda import _CODE, _followed, _launch
+from .cuda import _CODE, _followed, _hooked, _launch
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
+
+_DTYPE, _DEVICE = operator.attrgetter("dtype"), torch.Tensor.get_device
 
 # ScaoGatedFf: ten addresses, four row pitches, six numbers
 _ARGS = struct.Struct("@10P4q6i")
@@ -61,38 +65,50 @@ def _operands(tensors):
 
 
 def _forward(x, w_gate, w_up, act, train):
-    """(h, what the gradient reads or None, [the copy of each operand or None])."""
+    """(h, what the gradient reads or None, the copy of each operand or None, () without any)."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
     h = x.new_empty((rows, ff))
-    saved, copies = None, (None, None, None)
+    saved, copies = None, ()
     if train:
         saved = x.new_empty(L.scao_gated_ff_saved_bytes(rows, ff) >> 1)     # 16-bit places
     if rows:
-        ins, _ = _operands((x, w_gate, w_up))
+        ins, copied = _operands((x, w_gate, w_up))
         args = _ARGS.pack(ins[0][1], ins[1][1], ins[2][1], h.data_ptr(), saved.data_ptr() if train else 0,
                           0, 0, 0, 0, 0, ins[0][2], ins[1][2], ins[2][2], 0,
                           rows, d, ff, _CODE[x.dtype], act, 0)
         _launch("scao_gated_ff_forward", x.get_device(), L.scao_gated_ff_forward, args)
-        copies = [i[0] if i[3] else None for i in ins]
+        if copied and train:
+            copies = [i[0] if i[3] else None for i in ins]
     return h, saved, copies
+
+
+def _from_hooks(dh, ins, saved, places, copies):
+    """``saved`` where the kernels can read it; raises where hooks handed back something else
+    than was saved."""
+    (x, w_gate, w_up), kept = ins, (dh, *ins, saved)
+    if copies:
+        kept += tuple(c for c in copies if c is not None)
+    good = len(set(map(_DTYPE, kept))) == 1 == len(set(map(_DEVICE, kept))) and saved.numel() == places and \
+        dh.shape == (x.shape[0], w_gate.shape[0]) and w_gate.shape == w_up.shape and x.shape[1] == w_gate.shape[1]
+    for t, c in zip(ins, copies):
+        good = good and (c is None or c.shape == (t.shape[0], (t.shape[1] + 63) & ~63))
+    if not good:
+        raise RuntimeError("gated_ff: a saved tensor came back with another size, type or device")
+    return saved.clone(memory_format=torch.contiguous_format) \
+        if saved.data_ptr() & 15 or not saved.is_contiguous() else saved
 
 
 def _backward(x, w_gate, w_up, saved, dh, act, need_x, need_w, copies):
     """(dx, dw_gate, dw_up), None where not needed."""
     L, rows, (ff, d) = _lib.lib(), x.shape[0], w_gate.shape
-    # hooks may have moved what was saved
-    like, kept = (dh.get_device(), dh.dtype), [x, w_gate, w_up, saved, *(c for c in copies if c is not None)]
-    if any((t.get_device(), t.dtype) != like for t in kept) or dh.shape != (rows, ff) or x.shape[1] != d or \
-            w_up.shape != (ff, d) or saved.numel() != L.scao_gated_ff_saved_bytes(rows, ff) >> 1 or \
-            any(c is not None and c.shape != (t.shape[0], (d + 63) & ~63) for t, c in zip(kept, copies)):
-        raise RuntimeError("gated_ff: a saved tensor came back with another size, type or device")
-    if saved.data_ptr() & 15 or not saved.is_contiguous():
-        saved = saved.clone(memory_format=torch.contiguous_format)
     dx = x.new_empty((rows, d)) if need_x else None
     new = x.new_empty if rows else x.new_zeros
     dwg, dwu = (new((ff, d)), new((ff, d))) if need_w else (None, None)
     if rows:
-        ins, _ = _operands([t if c is None else c for t, c in zip((x, w_gate, w_up), copies)])
+        ins = (x, w_gate, w_up)
+        if copies:
+            ins = [t if c is None else c for t, c in zip(ins, copies)]
+        ins, _ = _operands(ins)
         if dh.stride(1) != 1:
             dh = dh.contiguous()
         ws = x.new_empty((L.scao_gated_ff_workspace_bytes(rows, d, ff, need_x | need_w << 1) + 1) >> 1)
@@ -121,15 +137,18 @@ class _GatedFF(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act):
         h, saved, copies = _forward(x, w_gate, w_up, act, True)
-        ctx.act = act
+        ctx.act, ctx.hooked = act, _hooked()
         ctx.save_for_backward(x, w_gate, w_up, saved, *copies)
         return h
 
     @staticmethod
     def backward(ctx, dh):
         need, (x, w_gate, w_up, saved, *copies) = ctx.needs_input_grad, ctx.saved_tensors
+        if ctx.hooked:
+            places = _lib.lib().scao_gated_ff_saved_bytes(dh.shape[0], dh.shape[1]) >> 1
+            saved = _from_hooks(dh, (x, w_gate, w_up), saved, places, copies)
         grads = _backward(x, w_gate, w_up, saved, dh, ctx.act, need[0], need[1] or need[2], copies)
-        if torch.is_grad_enabled() or _followed():
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0:
             grads = [None if g is None else _Once.apply(g, x, w_gate, w_up, dh) for g in grads]
         return *grads, None
 

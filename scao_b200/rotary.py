@@ -23,9 +23,10 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from .cuda import _CODE, _followed, _launch
+from .cuda import _CODE, _followed, _hooked, _launch
 
 MAX_DIM = 512
 
@@ -179,7 +180,7 @@ class _Turn(torch.autograd.Function):
     def forward(ctx, how, positions, q, k):
         ctx.how = how
         if positions is not None:
-            ctx.places = (positions.get_device(), positions.dtype, positions.shape)
+            ctx.places = (positions.get_device(), positions.dtype, positions.shape) if _hooked() else None
             ctx.save_for_backward(positions)
         ctx.set_materialize_grads(False)
         rotary, inverse, start, index = how
@@ -190,11 +191,12 @@ class _Turn(torch.autograd.Function):
         rotary, inverse, start, index = ctx.how
         saved = ctx.saved_tensors
         positions = saved[0] if saved else None
-        if positions is not None and (positions.get_device(), positions.dtype, positions.shape) != ctx.places:
+        if positions is not None and ctx.places is not None and \
+                ctx.places != (positions.get_device(), positions.dtype, positions.shape):
             raise RuntimeError("rotary: the positions came back with another size, type or device")
         _, _, need_q, need_k = ctx.needs_input_grad
         gq, gk = gq if need_q else None, gk if need_k else None
-        if torch.is_grad_enabled() or _followed():          # differentiable again
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0:   # differentiable again
             gq, gk = _Turn.apply((rotary, not inverse, start, index), positions, gq, gk)
         else:
             gq, gk = _run(rotary, not inverse, positions, start, index, (gq, gk))
