@@ -424,8 +424,8 @@ SCAO_API int scao_divc_check(const float* x, const float* c, int n, int* mismatc
 SCAO_API int64_t scao_grad_norm_workspace_bytes(int n);
 SCAO_API int scao_grad_norm(const int64_t* table, int n, int kind, void* workspace,
                             float* total, void* stream);
-/* g <- g min(1, max_norm / (*total + 1e-6)) for every gradient, rounded to
- * its type once; nothing is written where the factor is 1.  The gradients
+/* g <- g min(1, max_norm / (*total + 1e-6)) for every gradient, in 32 bits,
+ * then rounded to its type; nothing is written where the factor is 1.  The gradients
  * must not share memory (scao_grads_overlap, host only: 1 if they do, -1 for
  * a bad table).                                                            */
 SCAO_API int scao_grad_clip(const int64_t* table, int n, double max_norm, const float* total,

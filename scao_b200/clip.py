@@ -1,11 +1,13 @@
 """Global gradient norm and clipping, over any number of gradients in two launches.
 
-``clip_grad_norm_``, ``get_total_norm`` and ``clip_grads_with_norm_`` take what the
-functions of the same names in ``torch.nn.utils`` take (norms of order 1, 2 and inf)
-and return the norm as a float32 scalar on the gradients' device; nothing waits for
-the GPU.  Gradients may mix float32, bfloat16 and float16, sizes and alignments.
+``clip_grad_norm_``, ``get_total_norm`` and ``clip_grads_with_norm_`` do what the
+functions of the same names in ``torch.nn.utils`` do and return the norm as a float32
+scalar on the gradients' device; nothing waits for the GPU.  Refused, where those take it:
+norms of other orders than 1, 2 and inf, float64 and sparse gradients, gradients on the
+CPU or on several devices, gradients that share memory, a negative ``max_norm``, and the
+argument ``foreach``.  Gradients may mix float32, bfloat16 and float16, sizes and alignments.
 Sums are held in 64 bits over the whole range of float32, the same inputs give the
-same bits, and each scaled value is rounded once.  Gradients within the threshold are
+same bits, and each value is scaled in 32 bits and rounded to its type.  Gradients within the threshold are
 not written (strided ones that do not fill a range of memory are: with their own values).  CUDA tensors of one device only; errors raise.
 """
 from __future__ import annotations

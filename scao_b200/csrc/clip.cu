@@ -249,7 +249,8 @@ SCAO_DEV void scale_item(const Item& w, float c) {
 
 // The norm from `n_partial` partials, or `total_in`; block 0 writes it to
 // `total_out` where that is set.  Then c (formed in 64 bits, rounded to 32
-// once) and the scaling: one rounding of c g to the gradient's type.
+// once) and the scaling: c g in 32 bits, rounded then to the gradient's type (in 16 bits a
+// second rounding, of 2^-24, which moves a result only where the first falls on a border).
 template <int MAXT>
 __global__ void __launch_bounds__(CT, CBLOCKS)
 grad_scale_kernel(const __grid_constant__ GradTab<MAXT> tab, const double* __restrict__ partial,

@@ -21,11 +21,13 @@
 //
 // Few rows without a gradient take ff_skinny_kernel.
 //
-// Measured, M x d x F = 4096 x 2048 x 8192 in bf16 (275 GFLOP a projection pair): forward 163
-// us (1.69 PFLOP/s; a library product of the size, without activation, 166), 176 when g
-// and u are kept; pointwise 68 us (5.9 TB/s); both gradient products 340 us (1.62 PFLOP/s;
-// two library products 344).  Bound by the tensor cores at the clock that their power
-// leaves them (1.6 of 1.9 GHz): 77 to 86 % of their cycles.
+// Measured, M x d x F = 4096 x 2048 x 8192 in bf16 (275 GFLOP a projection pair), two calls
+// in a graph on a card that is not yet at its power cap: forward 167 us (1.65 PFLOP/s; a
+// library product of the size, without activation, 170), 186 when g and u are kept;
+// pointwise 68 us (5.9 TB/s); both gradient products 335 us (1.64 PFLOP/s; two library
+// products 350).  Bound by the tensor cores at the clock that their power leaves them (1.6 of
+// 1.9 GHz): 77 to 86 % of their cycles.  In a program's loop, at the cap (980 W, 1.40 to 1.55
+// GHz), the same take 206, 229 and 420 us, the three library products 211 + 209 + 216.
 #include <cuda.h>
 #include <string.h>
 

@@ -4,7 +4,8 @@
 
 ``x`` is (..., d), the weights are (ff, d) as ``torch.nn.Linear`` keeps them, h is
 (..., ff), all bfloat16 or all float16 (under CUDA autocast they are cast to its type)
-with 32-bit sums.  The activation is "silu", "gelu" or "gelu_tanh".  Both projections,
+with 32-bit sums; the weights' gradients have the weights' type (under autocast they are
+rounded to its type first and widened).  float32 without autocast raises.  The activation is "silu", "gelu" or "gelu_tanh".  Both projections,
 the activation and the product are one kernel; where a gradient will be taken it also
 keeps both projections' results in 24 bits (6 bytes for each value of h, in whole blocks
 of 128 rows x 128 columns: one row keeps what 128 do).
