@@ -17,10 +17,11 @@ from array import array
 from operator import attrgetter
 
 import torch
+from torch._C import _is_tracing
 from torch.autograd import forward_ad
 
 from . import _lib
-from .cuda import _CODE, _followed, _launch
+from .cuda import _CODE, _launch
 
 _KIND = {1.0: 0, 2.0: 1, math.inf: 2}
 _DTYPES = set(_CODE)
@@ -105,7 +106,9 @@ def _table(tensors, write):
     device number).  Strided gradients that are not dense are packed for the call; tensors
     that will be written must not share memory."""
     n, index = len(tensors), tensors[0].get_device()
-    if _followed() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if _is_tracing():
+        raise RuntimeError("the gradients' norm and clipping cannot be traced")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError("gradients with forward-mode tangents are not clipped")
     get, dtypes = torch.Tensor, set(map(_DTYPE, tensors))
     if index < 0 or not dtypes <= _DTYPES or set(map(get.get_device, tensors)) != {index} or \

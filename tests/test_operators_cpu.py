@@ -189,6 +189,16 @@ def test_c_entries_refuse_misaligned_addresses():
         assert L.scao_rotary(ctypes.byref(a), None) == 1, (pos, wide)
 
 
+@pytest.mark.filterwarnings("ignore")
+def test_clip_refuses_traces():
+    """torch.jit.trace would record the norm as it was allocated."""
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(lambda g: get_total_norm([g]), torch.ones(3), check_trace=False)
+    p = param(torch.ones(3))
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(lambda g: clip_grad_norm_([p], 1.0) * g, torch.ones(3), check_trace=False)
+
+
 @pytest.mark.parametrize("pre_dispatch", [False, True])
 def test_fx_traces_are_refused(pre_dispatch):
     from torch.fx.experimental.proxy_tensor import make_fx
