@@ -1210,7 +1210,9 @@ extern "C" int scao_gated_ff_plan(int rows, int d, int ff, int which, int32_t* o
     if (rows < 1 || d < 1 || ff < 1 || which < 0 || which > 3 || !out) return SCAO_ERR_ARG;
     if (which == 0) {
         out[0] = plan_forward(rows, d, ff);
-        out[1] = (int32_t)tiles_of(rows, ff, tile_rows(out[0]), tile_cols(out[0]) / 2);
+        const int64_t items = tiles_of(rows, ff, tile_rows(out[0]), tile_cols(out[0]) / 2);
+        if (items > 1 << 30) return SCAO_ERR_ARG;
+        out[1] = (int32_t)items;
         out[2] = out[3] = 1;
     } else {
         const FfPlan& p = plan_backward(rows, d, ff, which & 1, which & 2);

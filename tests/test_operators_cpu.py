@@ -366,6 +366,7 @@ def test_gated_ff_plan_checks():
     for args in ((0, 8, 8, 3), (8, 0, 8, 3), (8, 8, -1, 0), (8, 8, 8, 4), (8, 8, 8, -1)):
         assert L.scao_gated_ff_plan(*args, out) == 1, args
     assert L.scao_gated_ff_plan(8, 8, 8, 3, None) == 1
+    assert L.scao_gated_ff_plan((1 << 31) - 1, 8, 1 << 22, 0, out) == 1        # more tiles than a launch takes
 
 
 # ----------------------------------------------------------------- the model
