@@ -14,7 +14,8 @@
 //              into one accumulator, the weights read MN-major as they lie; dWg and dWu
 //              contract over the rows with both operands MN-major: nothing is transposed
 //              in memory.  dg and du come from a pointwise pass (ff_pointwise_kernel),
-//              rounded to 16 bits as operands of the tensor cores.
+//              rounded to 16 bits as operands of the tensor cores (in float16 infinite
+//              beyond 65504, as dh * u would be in that type).
 // That pass reads g and u as the forward pass kept them, in 24 bits: in 16 their rounding
 // would come beside those of dg, du and the result, and put the gradients' error at 1.8
 // instead of 1.4 roundings (of either type; 32 bits would not lower it).
